@@ -340,6 +340,45 @@ def attn_chunk_staged_gated(q, out, gate, n_heads, n_kv, head_dim, pos0, tokens,
         _lib.check("chunk_attention", rc)
 
 
+# ---- speculation with a tree of drafted tokens ---------------------------------------------------
+
+def attn_tree_workspace_bytes(n_heads, n_kv, head_dim, nodes, slots) -> int:
+    return int(_lib.load().hipml_attn_tree_workspace_bytes(n_heads, n_kv, head_dim, nodes, slots))
+
+
+def attn_tree(pos, parents, q, k_cache, v_cache, out, n_heads, n_kv, head_dim, stride, scale, nodes, slots,
+              kv_slot_bytes, workspace, kv_dtype=1):
+    """Attention of every slot's drafted nodes: the prefix, the node's ancestors and itself.
+
+    pos [slots][2] = (prefix rows, prefix and drafted rows), parents [slots][nodes] (-1: none), q and out f32
+    [slots][nodes][n_heads*head_dim]; kv_dtype 0 f32, 1 q8_0, 2 q4_0."""
+    rc = _c.attn_tree(kv_dtype, pos, parents, q, k_cache, v_cache, out, n_heads, n_kv, head_dim, stride, scale, nodes,
+                      slots, kv_slot_bytes, workspace,
+                      0 if workspace is None else workspace.numel() * workspace.element_size())
+    if rc:
+        _lib.check("attn_tree", rc)
+
+
+def tree_verify(pos, parents, tokens, target, draft, uniform, path, count, next_token, nodes, slots, vocab,
+                row_stride=None):
+    """Which drafted nodes are kept and the token that follows them, from target and draft probabilities
+    [slots][nodes][vocab] (draft None: looked up) and uniform [slots][nodes] (0: the next token's, i: node i's trial).
+
+    Writes path [slots][nodes] (kept nodes, then -1), count [slots] and next_token [slots]."""
+    rc = _c.tree_verify(pos, parents, tokens, target, draft, uniform, path, count, next_token, nodes, slots, vocab,
+                        vocab if row_stride is None else row_stride)
+    if rc:
+        _lib.check("tree_verify", rc)
+
+
+def kv_path_keep(pos, path, count, k_caches, v_caches, n_kv, head_dim, stride, nodes, slots, kv_slot_bytes, kv_dtype=1):
+    """In the caches of all layers (sequences of tensors) the kept path's rows base + path[i] become rows base + i."""
+    rc = _c.kv_path_keep(kv_dtype, pos, path, count, k_caches, v_caches, n_kv, head_dim, stride, nodes, slots,
+                         kv_slot_bytes)
+    if rc:
+        _lib.check("kv_path_keep", rc)
+
+
 def check_device_status() -> int:
     """Synchronises the current stream; raises if a kernel's bounded wait ran out."""
     st = C.c_int(0)

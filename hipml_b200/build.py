@@ -26,6 +26,9 @@ SOURCES = [
     "attn_chunk_scalar.cu",
     "attn_chunk_small.cu",
     "attn_chunk_tc.cu",
+    "attn_tree.cu",
+    "tree_verify.cu",
+    "kv_path.cu",
     "launchers.cu",
 ]
 

@@ -1,0 +1,280 @@
+// Attention of a tree of drafted tokens over a cache (f32, q8_0, q4_0; several slots), on the CUDA cores, and the fold of
+// the runs' partials. For node i of a slot, with `base` prefix rows and the drafted rows behind them:
+//     out_i = sum_j w_ij v_j / sum_j w_ij,  w_ij = 2^(scale log2(e) q_i . k_j - m_i),
+//     j over [0, base) and base + {i and its ancestors}.
+// No counterpart in the reference, whose verify columns are a chain (crates/hipml-kernels/src/launch_kv.rs:320-400).
+//
+// This kernel takes the head sizes and alignments that the tensor-core kernel does not. A CTA has 32 query rows, four to a
+// warp, and walks its run 32 cache rows at a time: the tile is dequantised once to f32 in shared memory for all of them
+// (scores: lane = cache row; values: lane = dims), so the cache is read once per 32 query rows and the products are plain
+// f32 FMAs, which bound it.
+#include "q8_pack.cuh"
+#include "tree.cuh"
+
+namespace hipml {
+
+namespace {
+
+constexpr int kRows = 32, kWarpRows = 4, kWarps = 8, kKeys = 32;
+
+// Values [32 * blk, +32) of one KV head's cache row, as f32 into dst[0 .. 31].
+__device__ __forceinline__ void load_block(const TreeParams &p, const unsigned char *cache, int kvh, int row, int blk,
+                                           float *dst) {
+    if (p.kv_dtype == 0) {
+        const float *src = reinterpret_cast<const float *>(cache) + ((size_t)row * p.n_kv + kvh) * p.head_dim + 32 * blk;
+#pragma unroll
+        for (int j = 0; j < 32; j++) dst[j] = src[j];
+    } else if (p.kv_dtype == 1) {
+        const unsigned short *src = reinterpret_cast<const unsigned short *>(
+            cache + q8_row_offset(kvh, p.stride, row, p.head_dim) + (size_t)blk * kQ8BlockBytes);
+        const float d = half_bits_to_float(src[0]);
+#pragma unroll
+        for (int j = 0; j < 16; j++) {
+            const unsigned short w = src[1 + j];
+            dst[2 * j] = d * (float)(signed char)(w & 0xff);
+            dst[2 * j + 1] = d * (float)(signed char)(w >> 8);
+        }
+    } else {
+        const unsigned short *src = reinterpret_cast<const unsigned short *>(
+            cache + q4_row_offset(kvh, p.stride, row, p.head_dim) + (size_t)blk * kQ4BlockBytes);
+        const float d = half_bits_to_float(src[0]);
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+            const unsigned short w = src[1 + j];
+            dst[2 * j] = d * ((float)(w & 15) - 8.0f);
+            dst[2 * j + 1] = d * ((float)((w >> 8) & 15) - 8.0f);
+            dst[2 * j + 16] = d * ((float)((w >> 4) & 15) - 8.0f);
+            dst[2 * j + 17] = d * ((float)(w >> 12) - 8.0f);
+        }
+    }
+}
+
+// grid as tree_grid, block 256, kB = head_dim / 32.
+template <int kB>
+__global__ void __launch_bounds__(256) attn_tree_scalar(TreeParams p) {
+    constexpr int kD = 32 * kB, kPitch = kD + 1;
+    extern __shared__ float smem[];
+    float *const ks = smem, *const vs = ks + kKeys * kPitch, *const qs = vs + kKeys * kPitch;
+    __shared__ TreeItem s_item;
+    __shared__ int s_parents[kTreeNodes];
+    __shared__ unsigned s_sees[kRows][kTreeWords];
+    griddep_launch();
+    griddep_wait();
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    if (warp == 0) {
+        const TreeItem it = tree_item(p, tree_quota(p), blockIdx.x);
+        if (lane == 0) s_item = it;
+    }
+    __syncthreads();
+    const TreeItem it = s_item;
+    if (it.slot < 0) return;
+    const int rows = min(kRows, it.live * p.group - it.tile * kRows);
+    const int len = it.base + it.live;
+    const int lo = it.run * it.quota * kTreeKeyTile, hi = min(lo + it.quota * kTreeKeyTile, len);
+    for (int i = tid; i < it.live; i += 256) s_parents[i] = p.parents[(size_t)it.slot * p.nodes + i];
+    const size_t slot_row = (size_t)it.slot * p.nodes;
+    // a row of the tile as a row of q and out, in heads
+    auto head_row = [&](int r) {
+        const int at = it.tile * kRows + r, node = at / p.group;
+        return (slot_row + node) * p.n_heads + it.kvh * p.group + (at - node * p.group);
+    };
+    for (int i = tid; i < kRows * kD; i += 256) {
+        const int r = i / kD;
+        qs[i] = r < rows ? p.q[head_row(r) * kD + (i - r * kD)] * p.scale_log2 : 0.0f;
+    }
+    __syncthreads();
+    if (tid < rows) {
+        unsigned words[kTreeWords];
+        tree_ancestors(s_parents, (it.tile * kRows + tid) / p.group, words, p.status);
+#pragma unroll
+        for (int w = 0; w < kTreeWords; w++) s_sees[tid][w] = words[w];
+    }
+    const unsigned char *const kc = p.k + (size_t)it.slot * p.slot_bytes, *const vc = p.v + (size_t)it.slot * p.slot_bytes;
+    float acc[kWarpRows][kB], m[kWarpRows], l[kWarpRows];
+#pragma unroll
+    for (int a = 0; a < kWarpRows; a++) {
+        m[a] = -INFINITY;
+        l[a] = 0.0f;
+#pragma unroll
+        for (int b = 0; b < kB; b++) acc[a][b] = 0.0f;
+    }
+    for (int k0 = lo; k0 < hi; k0 += kKeys) {
+        __syncthreads();
+        for (int i = warp; i < 2 * kB; i += kWarps) {   // lane = cache row: the stores fall into different banks
+            const int blk = i % kB;
+            float *const dst = (i < kB ? ks : vs) + lane * kPitch + 32 * blk;
+            if (k0 + lane < hi) {
+                load_block(p, i < kB ? kc : vc, it.kvh, k0 + lane, blk, dst);
+            } else {
+#pragma unroll
+                for (int j = 0; j < 32; j++) dst[j] = 0.0f;
+            }
+        }
+        __syncthreads();
+        float s[kWarpRows] = {0.0f, 0.0f, 0.0f, 0.0f};
+        const float *const krow = ks + lane * kPitch, *const qrow = qs + warp * kWarpRows * kD;
+#pragma unroll 4
+        for (int d = 0; d < kD; d += 4) {
+            const float k0v = krow[d], k1v = krow[d + 1], k2v = krow[d + 2], k3v = krow[d + 3];
+#pragma unroll
+            for (int a = 0; a < kWarpRows; a++) {
+                const float4 x = *reinterpret_cast<const float4 *>(qrow + a * kD + d);
+                s[a] = fmaf(x.x, k0v, fmaf(x.y, k1v, fmaf(x.z, k2v, fmaf(x.w, k3v, s[a]))));
+            }
+        }
+        unsigned seen[kWarpRows];   // bit j: the row sees cache row k0 + j
+#pragma unroll
+        for (int a = 0; a < kWarpRows; a++) {
+            const int r = warp * kWarpRows + a, drafted = k0 + lane - it.base;
+            bool sees = r < rows && k0 + lane < hi;
+            if (sees && drafted >= 0) sees = s_sees[r][drafted >> 5] >> (drafted & 31) & 1;
+            seen[a] = __ballot_sync(0xffffffffu, sees);
+            // (a row that sees nothing of these keeps what it has: -inf - -inf must not be formed)
+            const float mine = sees ? s[a] : -INFINITY;
+            const float m_new = fmaxf(m[a], warp_max(mine));
+            const float ref = m_new == -INFINITY ? 0.0f : m_new;
+            const float corr = exp2f(m[a] - ref);
+            s[a] = sees ? exp2f(mine - ref) : 0.0f;
+            l[a] = l[a] * corr + warp_sum(s[a]);
+            m[a] = m_new;
+#pragma unroll
+            for (int b = 0; b < kB; b++) acc[a][b] *= corr;
+        }
+#pragma unroll 4
+        for (int j = 0; j < kKeys; j++) {
+            float x[kB];
+#pragma unroll
+            for (int b = 0; b < kB; b++) x[b] = vs[j * kPitch + 32 * b + lane];
+#pragma unroll
+            for (int a = 0; a < kWarpRows; a++) {
+                const float w = __shfl_sync(0xffffffffu, s[a], j);
+                if (seen[a] >> j & 1) {   // what a row does not see may hold anything
+#pragma unroll
+                    for (int b = 0; b < kB; b++) acc[a][b] = fmaf(w, x[b], acc[a][b]);
+                }
+            }
+        }
+    }
+#pragma unroll
+    for (int a = 0; a < kWarpRows; a++) {
+        const int r = warp * kWarpRows + a;
+        if (r >= rows) break;
+        const bool whole = it.runs == 1;
+        const size_t part = (size_t)blockIdx.x * kRows + r;
+        float *const dst = whole ? p.out + head_row(r) * kD : p.part_acc + part * kD;
+        const float inv = whole ? 1.0f / l[a] : 1.0f;
+#pragma unroll
+        for (int b = 0; b < kB; b++) dst[32 * b + lane] = acc[a][b] * inv;
+        if (!whole && lane == 0) {
+            p.part_ml[2 * part] = m[a];
+            p.part_ml[2 * part + 1] = l[a];
+        }
+    }
+}
+
+// The runs of a query row, folded: grid (n_heads * nodes, slots), 256 threads; a column of four dims has 1024 / head_dim
+// threads, which take the runs in turn.
+__global__ void __launch_bounds__(256) attn_tree_fold(TreeParams p) {
+    __shared__ int s_quota, s_first;
+    __shared__ float s_max[8];
+    __shared__ float4 s_sum[256];
+    __shared__ float s_den[256];
+    griddep_launch();
+    griddep_wait();
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int slot = blockIdx.y, node = blockIdx.x / p.n_heads, head = blockIdx.x - node * p.n_heads;
+    const TreeSlot t = tree_slot(p.pos, slot, p.stride, p.nodes);
+    if (node >= t.live) return;
+    if (warp == 0) {
+        const int quota = tree_quota(p);
+        int first = 0;
+        for (int s = lane; s < slot; s += 32) first += tree_ctas(p, tree_slot(p.pos, s, p.stride, p.nodes), quota);
+        first = __reduce_add_sync(0xffffffffu, first);
+        if (lane == 0) {
+            s_quota = quota;
+            s_first = first;
+        }
+    }
+    __syncthreads();
+    const int runs = div_up_int(t.base + t.live, kTreeKeyTile * s_quota);
+    if (runs == 1) return;   // (written by the run itself)
+    const int kvh = head / p.group, at = node * p.group + head - kvh * p.group;
+    const int tile = at / p.tile_rows, r = at - tile * p.tile_rows;
+    const int tiles = div_up_int(t.live * p.group, p.tile_rows);
+    const size_t first = (size_t)s_first + (size_t)(kvh * tiles + tile) * runs;
+    const float2 *const ml = reinterpret_cast<const float2 *>(p.part_ml) + first * p.tile_rows + r;
+    float big = -INFINITY;
+    for (int j = tid; j < runs; j += 256) big = fmaxf(big, ml[(size_t)j * p.tile_rows].x);
+    big = warp_max(big);
+    if (lane == 0) s_max[warp] = big;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < 8; w++) big = fmaxf(big, s_max[w]);
+    const int cols = p.head_dim / 4, groups = 256 / cols;
+    const int col = tid % cols, g = tid / cols;
+    float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    float den = 0.0f;
+    if (g < groups) {
+        const float4 *const acc = reinterpret_cast<const float4 *>(p.part_acc + (first * p.tile_rows + r) * p.head_dim) + col;
+        const size_t step = (size_t)p.tile_rows * cols;
+#pragma unroll 4
+        for (int j = g; j < runs; j += groups) {
+            const float2 x = ml[(size_t)j * p.tile_rows];
+            const float4 a = acc[j * step];
+            const float w = x.x == -INFINITY ? 0.0f : exp2f(x.x - big);   // (a run of which the row sees nothing)
+            sum.x = fmaf(a.x, w, sum.x);
+            sum.y = fmaf(a.y, w, sum.y);
+            sum.z = fmaf(a.z, w, sum.z);
+            sum.w = fmaf(a.w, w, sum.w);
+            den = fmaf(x.y, w, den);
+        }
+    }
+    s_sum[tid] = sum;
+    s_den[tid] = den;
+    __syncthreads();
+    if (g == 0) {
+        for (int i = 1; i < groups; i++) {
+            const float4 a = s_sum[i * cols + col];
+            sum.x += a.x;
+            sum.y += a.y;
+            sum.z += a.z;
+            sum.w += a.w;
+            den += s_den[i * cols + col];
+        }
+        const float inv = 1.0f / den;
+        reinterpret_cast<float4 *>(p.out + (((size_t)slot * p.nodes + node) * p.n_heads + head) * p.head_dim)[col] =
+            make_float4(sum.x * inv, sum.y * inv, sum.z * inv, sum.w * inv);
+    }
+}
+
+template <int kB>
+int launch_scalar(cudaStream_t stream, const TreeParams &p) {
+    constexpr int kD = 32 * kB;
+    constexpr size_t kSmem = (2 * (size_t)kKeys * (kD + 1) + (size_t)kRows * kD) * sizeof(float);
+    if (kSmem > 48 * 1024) {   // (per device; setting it again is cheap beside a launch)
+        const cudaError_t e = cudaFuncSetAttribute(attn_tree_scalar<kB>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmem);
+        if (e != cudaSuccess) return (int)e;
+    }
+    return launch_pdl(attn_tree_scalar<kB>, dim3(p.grid), dim3(256), kSmem, stream, 1, p);
+}
+
+}  // namespace
+
+int launch_tree_scalar(cudaStream_t stream, const TreeParams &p) {
+    switch (p.head_dim / 32) {
+        case 1: return launch_scalar<1>(stream, p);
+        case 2: return launch_scalar<2>(stream, p);
+        case 3: return launch_scalar<3>(stream, p);
+        case 4: return launch_scalar<4>(stream, p);
+        case 5: return launch_scalar<5>(stream, p);
+        case 6: return launch_scalar<6>(stream, p);
+        case 7: return launch_scalar<7>(stream, p);
+        default: return launch_scalar<8>(stream, p);
+    }
+}
+
+int launch_tree_fold(cudaStream_t stream, const TreeParams &p) {
+    return launch_pdl(attn_tree_fold, dim3(p.n_heads * p.nodes, p.slots), dim3(256), 0, stream, 1, p);
+}
+
+}  // namespace hipml

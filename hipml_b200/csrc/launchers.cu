@@ -7,6 +7,7 @@
 #include <atomic>
 
 #include "params.cuh"
+#include "tree.cuh"
 
 using namespace hipml;
 
@@ -892,6 +893,142 @@ int hipml_attn_decode_cols_f32(hipml_stream_t stream, const float *q, const floa
     splits = splits < 1 ? 1 : (splits > 64 ? 64 : splits);
     return launch_decode_cols_f32(as_stream(stream), q, k_cache, v_cache, part_acc, part_ml, out,
                                   n_heads, n_kv, head_dim, n_ctx, pos0, rows, splits);
+}
+
+// ---- tree speculation ------------------------------------------------------------------
+
+static int check_tree(int kv_dtype, int n_kv, int head_dim, int stride, int nodes, int slots) {
+    if (kv_dtype < 0 || kv_dtype > 2) return fail(HIPML_ERR_INVALID_ARGUMENT, "unknown KV dtype %d", kv_dtype);
+    if (n_kv <= 0 || stride <= 0)
+        return fail(HIPML_ERR_INVALID_ARGUMENT, "n_kv %d / stride %d must be positive", n_kv, stride);
+    if (head_dim % 32 != 0 || head_dim < 32 || head_dim > 256)
+        return fail(HIPML_ERR_INVALID_ARGUMENT, "head_dim %d: must be 32..=256, multiple of 32", head_dim);
+    if (nodes < 1 || nodes > kTreeNodes)
+        return fail(HIPML_ERR_INVALID_ARGUMENT, "tree of %d nodes: must be 1..=%d", nodes, kTreeNodes);
+    if (slots < 1 || slots > 65535) return fail(HIPML_ERR_INVALID_ARGUMENT, "slots %d: must be 1..=65535", slots);
+    return 0;
+}
+
+// A slot's bytes must hold its rows, where there are several slots.
+static int check_slot_bytes(int kv_dtype, int n_kv, int head_dim, int stride, int slots, size_t kv_slot_bytes) {
+    const size_t row = kv_dtype == 0 ? (size_t)head_dim * 4 : (size_t)(head_dim / 32) * (kv_dtype == 1 ? 34 : 18);
+    if (slots > 1 && (kv_slot_bytes < row * n_kv * stride || kv_slot_bytes % (kv_dtype == 0 ? 4 : 2) != 0))
+        return fail(HIPML_ERR_INVALID_ARGUMENT, "%zu bytes a slot: %zu needed, a multiple of %d", kv_slot_bytes,
+                    row * n_kv * stride, kv_dtype == 0 ? 4 : 2);
+    return 0;
+}
+
+constexpr int kScalarTile = 32;
+
+size_t hipml_attn_tree_workspace_bytes(int n_heads, int n_kv, int head_dim, int nodes, int slots) {
+    if (check_heads(n_heads, n_kv, head_dim) || n_heads <= 0 || check_tree(0, n_kv, head_dim, 1, nodes, slots)) return 0;
+    const int grid = tree_grid(n_heads, n_kv, nodes, slots, kScalarTile, 2 * device_sms());
+    return grid < 0 ? 0 : (size_t)grid * kScalarTile * (head_dim + 2) * sizeof(float);
+}
+
+int hipml_attn_tree(hipml_stream_t stream, int kv_dtype, const int *pos, const int *parents, const float *q,
+                    const void *k_cache, const void *v_cache, float *out, int n_heads, int n_kv, int head_dim, int stride,
+                    float scale, int nodes, int slots, size_t kv_slot_bytes, void *workspace, size_t workspace_bytes) {
+    if (int e = check_tree(kv_dtype, n_kv, head_dim, stride, nodes, slots)) return e;
+    if (n_heads <= 0) return fail(HIPML_ERR_INVALID_ARGUMENT, "n_heads %d must be positive", n_heads);
+    if (int e = check_heads(n_heads, n_kv, head_dim)) return e;
+    if (int e = check_slot_bytes(kv_dtype, n_kv, head_dim, stride, slots, kv_slot_bytes)) return e;
+    if (!pos || !parents || !q || !k_cache || !v_cache || !out)
+        return fail(HIPML_ERR_INVALID_ARGUMENT, "tree attention: a tensor is missing");
+    if (((reinterpret_cast<size_t>(q) | reinterpret_cast<size_t>(out)) & 15) != 0)
+        return fail(HIPML_ERR_INVALID_ARGUMENT, "tree attention: q and out must be 16-byte aligned");
+    if (((reinterpret_cast<size_t>(k_cache) | reinterpret_cast<size_t>(v_cache)) & (kv_dtype == 0 ? 3 : 1)) != 0)
+        return fail(HIPML_ERR_INVALID_ARGUMENT, "tree attention: the caches must be %d-byte aligned", kv_dtype == 0 ? 4 : 2);
+    const size_t need = hipml_attn_tree_workspace_bytes(n_heads, n_kv, head_dim, nodes, slots);
+    if (need == 0) return fail(HIPML_ERR_INVALID_ARGUMENT, "tree attention: %d slots of %d nodes are too many", slots, nodes);
+    if (!workspace || workspace_bytes < need)
+        return fail(HIPML_ERR_WORKSPACE, "tree attention workspace: %zu bytes given, %zu needed", workspace_bytes, need);
+    if ((reinterpret_cast<size_t>(workspace) & 15) != 0)
+        return fail(HIPML_ERR_WORKSPACE, "tree attention workspace must be 16-byte aligned");
+    TreeParams p;
+    p.status = device_status_word();
+    if (!p.status) return launch_status();
+    p.pos = pos;
+    p.parents = parents;
+    p.q = q;
+    p.k = (const unsigned char *)k_cache;
+    p.v = (const unsigned char *)v_cache;
+    p.out = out;
+    p.n_heads = n_heads;
+    p.n_kv = n_kv;
+    p.group = n_heads / n_kv;
+    p.head_dim = head_dim;
+    p.stride = stride;
+    p.nodes = nodes;
+    p.slots = slots;
+    p.kv_dtype = kv_dtype;
+    p.scale_log2 = scale * kLog2e;
+    p.slot_bytes = kv_slot_bytes;
+    p.tile_rows = kScalarTile;
+    p.grid = tree_grid(n_heads, n_kv, nodes, slots, kScalarTile, 2 * device_sms());
+    p.part_acc = (float *)workspace;
+    p.part_ml = p.part_acc + (size_t)p.grid * p.tile_rows * head_dim;
+    if (int e = launch_tree_scalar(as_stream(stream), p)) return e;
+    return launch_tree_fold(as_stream(stream), p);
+}
+
+int hipml_tree_verify(hipml_stream_t stream, const int *pos, const int *parents, const int *tokens, const float *target,
+                      const float *draft, const float *uniform, int *path, int *count, int *next, int nodes, int slots,
+                      int vocab, long long row_stride) {
+    if (int e = check_tree(0, 1, 32, 1, nodes, slots)) return e;
+    if (vocab < 1 || vocab > kVerifyVocab)
+        return fail(HIPML_ERR_INVALID_ARGUMENT, "vocabulary of %d tokens: must be 1..=%d", vocab, kVerifyVocab);
+    if (row_stride < vocab)
+        return fail(HIPML_ERR_INVALID_ARGUMENT, "rows of %lld probabilities for %d tokens", row_stride, vocab);
+    if (!pos || !parents || !tokens || !target || !uniform || !path || !count || !next)
+        return fail(HIPML_ERR_INVALID_ARGUMENT, "tree verification: a tensor is missing");
+    VerifyParams p = {pos, parents, tokens, target, draft, uniform, path, count, next, device_status_word(),
+                      nodes, slots, vocab, row_stride};
+    if (!p.status) return launch_status();
+    return launch_tree_verify(as_stream(stream), p);
+}
+
+int hipml_kv_path_keep(hipml_stream_t stream, int kv_dtype, const int *pos, const int *path, const int *count,
+                       void *const *k_caches, void *const *v_caches, int layers, int n_kv, int head_dim, int stride,
+                       int nodes, int slots, size_t kv_slot_bytes) {
+    if (int e = check_tree(kv_dtype, n_kv, head_dim, stride, nodes, slots)) return e;
+    if (int e = check_slot_bytes(kv_dtype, n_kv, head_dim, stride, slots, kv_slot_bytes)) return e;
+    if (layers < 0) return fail(HIPML_ERR_INVALID_ARGUMENT, "layers %d", layers);
+    if (layers == 0) return 0;
+    if (!pos || !path || !count || !k_caches || !v_caches)
+        return fail(HIPML_ERR_INVALID_ARGUMENT, "kept path: a tensor is missing");
+    for (int i = 0; i < 2 * layers; i++) {
+        const void *const at = i < layers ? k_caches[i] : v_caches[i - layers];
+        if (!at || (reinterpret_cast<size_t>(at) & (kv_dtype == 0 ? 3 : 1)) != 0)
+            return fail(HIPML_ERR_INVALID_ARGUMENT, "kept path: cache %d is missing or not %d-byte aligned", i,
+                        kv_dtype == 0 ? 4 : 2);
+        for (int j = 0; j < i; j++)   // (its rows would be moved twice)
+            if (at == (j < layers ? k_caches[j] : v_caches[j - layers]))
+                return fail(HIPML_ERR_INVALID_ARGUMENT, "kept path: caches %d and %d are the same", j, i);
+    }
+    PathParams p;
+    p.pos = pos;
+    p.path = path;
+    p.count = count;
+    p.status = device_status_word();
+    if (!p.status) return launch_status();
+    p.n_kv = n_kv;
+    p.stride = stride;
+    p.nodes = nodes;
+    p.slot_bytes = slots > 1 ? (long long)kv_slot_bytes : 0;
+    p.row_bytes = kv_dtype == 0 ? head_dim * 4 : head_dim / 32 * (kv_dtype == 1 ? 34 : 18);
+    p.row_pitch = kv_dtype == 0 ? (long long)n_kv * p.row_bytes : p.row_bytes;
+    p.head_pitch = kv_dtype == 0 ? p.row_bytes : (long long)stride * p.row_bytes;
+    for (int l0 = 0; l0 < layers; l0 += kPathLayers) {
+        const int n = layers - l0 < kPathLayers ? layers - l0 : kPathLayers;
+        p.which = 2 * n;
+        for (int i = 0; i < n; i++) {
+            p.cache[2 * i] = (unsigned char *)k_caches[l0 + i];
+            p.cache[2 * i + 1] = (unsigned char *)v_caches[l0 + i];
+        }
+        if (int e = launch_kv_path_keep(as_stream(stream), p, slots)) return e;
+    }
+    return 0;
 }
 
 int hipml_set_decode_cta_slots(int slots) {

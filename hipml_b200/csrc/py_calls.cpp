@@ -14,6 +14,7 @@
 
 #include <tuple>
 #include <utility>
+#include <vector>
 
 #include "../../include/hipml_cuda.h"
 
@@ -106,6 +107,26 @@ struct From<Sections> {
     }
 };
 
+// Device pointers of a sequence of tensors.
+struct Pointers {
+    std::vector<void *> at;
+};
+template <>
+struct From<Pointers> {
+    static Pointers py(PyObject *o, bool &ok) {
+        Pointers r;
+        PyObject *items = PySequence_Tuple(o);
+        if (!items) {
+            ok = false;
+            return r;
+        }
+        const Py_ssize_t n = PyTuple_GET_SIZE(items);
+        for (Py_ssize_t i = 0; i < n && ok; i++) r.at.push_back(pointer_of(PyTuple_GET_ITEM(items, i), ok));
+        Py_DECREF(items);
+        return r;
+    }
+};
+
 // Nothing is converted once an argument has failed: Python must not be called with an exception set.
 template <class T>
 T take(PyObject *o, bool &ok) {
@@ -161,6 +182,17 @@ int front_append(hipml_stream_t stream, const float *qg, const float *k, const f
                                       tokens, stride, theta_base, eps);
 }
 
+// hipml_kv_path_keep: the caches are sequences, of equal length.
+int path_keep(hipml_stream_t stream, int kv_dtype, const int *pos, const int *path, const int *count, Pointers k,
+              Pointers v, int n_kv, int head_dim, int stride, int nodes, int slots, size_t kv_slot_bytes) {
+    // (a layer without one of its caches is refused there)
+    const size_t layers = k.at.size() > v.at.size() ? k.at.size() : v.at.size();
+    k.at.resize(layers, nullptr);
+    v.at.resize(layers, nullptr);
+    return hipml_kv_path_keep(stream, kv_dtype, pos, path, count, k.at.data(), v.at.data(), (int)layers, n_kv, head_dim,
+                              stride, nodes, slots, kv_slot_bytes);
+}
+
 #define CALL(name, fn) {name, (PyCFunction)(void (*)(void))Call<decltype(&fn), &fn>::py, METH_FASTCALL, nullptr}
 
 PyMethodDef kMethods[] = {
@@ -190,6 +222,9 @@ PyMethodDef kMethods[] = {
     CALL("norm_rope_chunk", hipml_norm_rope_chunk),
     CALL("q_gate", hipml_q_gate),
     CALL("attn_front_append_q8", front_append),
+    CALL("attn_tree", hipml_attn_tree),
+    CALL("tree_verify", hipml_tree_verify),
+    CALL("kv_path_keep", path_keep),
     {nullptr, nullptr, 0, nullptr},
 };
 

@@ -457,6 +457,58 @@ int hipml_attn_chunk_staged_gated(hipml_stream_t stream, const float *q, float *
                                   int tokens, float *part_acc, float *part_ml, int splits, int mode,
                                   int key_capacity, void *workspace, size_t workspace_bytes);
 
+/* ---- Speculation with a tree of drafted tokens (no counterpart in the reference, whose drafts are
+ * chains: hipml_attn_decode_cols) ----
+ * A slot's tree has up to `nodes` nodes (1..256). pos is device i32 [slots][2] = (base, base + live
+ * nodes), the step words of the other entries: the drafted rows lie behind the prefix, node i's in
+ * cache row base + i (append them with hipml_kv_encode_bulk, hipml_kv_append_cols_f32 or
+ * hipml_attn_front_append_q8). parents is device i32 [slots][nodes]: the parent of node i, an
+ * earlier node (< i), or -1. Nothing of a node past a slot's live ones is read or written, whatever
+ * the buffers hold there; lengths past the cache count as the cache. kv_dtype, caches and stride
+ * are those of hipml_attn_chunk (0 f32 [stride][n_kv*head_dim], 1 q8_0, 2 q4_0 head-major), slot s
+ * begins at byte s*kv_slot_bytes (any value where slots is 1). 1..65535 slots. A parent that is no
+ * earlier node ends that node's ancestors there and is reported by hipml_check_device_status as 41.
+ * All of it can be captured and replayed: lengths, trees and paths are read on the device. Calls that may
+ * overlap on the device must not share a workspace; nothing else is shared between calls.
+ *
+ * Attention of the drafted nodes in one call: node i sees cache rows [0, base), its own row and
+ * those of its ancestors. q and out are f32 [slots][nodes][n_heads*head_dim], 16-byte aligned. A row
+ * that a node does not see may hold anything, NaN and infinities too, without effect on it.
+ * workspace: hipml_attn_tree_workspace_bytes(...) bytes on 16 (0: the arguments are refused; it
+ * depends on the current device's SMs). */
+size_t hipml_attn_tree_workspace_bytes(int n_heads, int n_kv, int head_dim, int nodes, int slots);
+int hipml_attn_tree(hipml_stream_t stream, int kv_dtype, const int *pos, const int *parents,
+                    const float *q, const void *k_cache, const void *v_cache, float *out, int n_heads,
+                    int n_kv, int head_dim, int stride, float scale, int nodes, int slots,
+                    size_t kv_slot_bytes, void *workspace, size_t workspace_bytes);
+
+/* Which nodes are kept, and the token that follows them. Node 0 is the last token of the sequence
+ * (always kept), tokens i32 [slots][nodes] the drafted token of every other node, target f32 rows of
+ * `vocab` probabilities, row s*nodes + i (rows row_stride floats apart) the target's distribution
+ * behind node i, draft (NULL: the drafted tokens were looked up, not drawn) likewise the drafter's.
+ * uniform f32 [slots][nodes] are numbers of [0, 1). From node 0 on, with r = the target row, the
+ * children of the last kept node are tried in the order of their indexes: child c with token x is
+ * kept where uniform[c] * q(x) < r(x), q being the draft row of its parent (without draft rows 1 at
+ * x, 0 elsewhere); otherwise r becomes max(r - q, 0) over its sum (and stays where that is 0). Where
+ * no child is kept, `next` is the lowest token whose running sum of r exceeds uniform[0] times
+ * the whole (the last token with r > 0 where rounding leaves none; -1 where r has no mass). path i32
+ * [slots][nodes] receives the kept nodes in order, then -1; count i32 [slots] how many. Outputs of a
+ * slot without live nodes stay as they are. Sums are in 64 bits. What is no probability (NaN,
+ * negative, infinite) counts as 0; a child whose parent is no earlier node or whose token is not in
+ * the vocabulary is never kept (device status 41). vocab 1..1048576. */
+int hipml_tree_verify(hipml_stream_t stream, const int *pos, const int *parents, const int *tokens,
+                      const float *target, const float *draft, const float *uniform, int *path,
+                      int *count, int *next, int nodes, int slots, int vocab, long long row_stride);
+
+/* The kept path's cache rows move together behind the prefix: in every cache of `layers` layers row
+ * base + path[i] becomes row base + i, i < count (path and count as hipml_tree_verify leaves them; the
+ * other rows stay). k_caches and v_caches are HOST arrays of `layers` device pointers, all different.
+ * A path must ascend and stay among the live nodes: otherwise the slot is left as it was (device status 42).
+ * One launch for up to 64 layers; cache addresses are taken at the call. */
+int hipml_kv_path_keep(hipml_stream_t stream, int kv_dtype, const int *pos, const int *path,
+                       const int *count, void *const *k_caches, void *const *v_caches, int layers,
+                       int n_kv, int head_dim, int stride, int nodes, int slots, size_t kv_slot_bytes);
+
 /* Tuning and test knobs of the decode path (no counterpart in the reference).
  * hipml_set_decode_cta_slots: how many CTAs of the tensor-core decode kernel one round of the
  * device holds (default 0 = 2 per SM of the current device); a process that shares the GPU
