@@ -27,6 +27,7 @@ SOURCES = [
     "attn_chunk_small.cu",
     "attn_chunk_tc.cu",
     "attn_tree.cu",
+    "attn_tree_tc.cu",
     "tree_verify.cu",
     "kv_path.cu",
     "launchers.cu",

@@ -15,7 +15,7 @@ namespace hipml {
 
 namespace {
 
-constexpr int kRows = 32, kWarpRows = 4, kWarps = 8, kKeys = 32;
+constexpr int kRows = kTreeScalarRows, kWarpRows = 4, kWarps = 8, kKeys = 32;
 
 // Values [32 * blk, +32) of one KV head's cache row, as f32 into dst[0 .. 31].
 __device__ __forceinline__ void load_block(const TreeParams &p, const unsigned char *cache, int kvh, int row, int blk,

@@ -918,12 +918,19 @@ static int check_slot_bytes(int kv_dtype, int n_kv, int head_dim, int stride, in
     return 0;
 }
 
-constexpr int kScalarTile = 32;
+// CTAs of the two kernels of tree attention: one or two to an SM.
+static int tree_grid_of(bool tensor_core, int n_heads, int n_kv, int nodes, int slots) {
+    return tensor_core ? tree_grid(n_heads, n_kv, nodes, slots, kTreeTcRows, device_sms())
+                       : tree_grid(n_heads, n_kv, nodes, slots, kTreeScalarRows, 2 * device_sms());
+}
 
 size_t hipml_attn_tree_workspace_bytes(int n_heads, int n_kv, int head_dim, int nodes, int slots) {
     if (check_heads(n_heads, n_kv, head_dim) || n_heads <= 0 || check_tree(0, n_kv, head_dim, 1, nodes, slots)) return 0;
-    const int grid = tree_grid(n_heads, n_kv, nodes, slots, kScalarTile, 2 * device_sms());
-    return grid < 0 ? 0 : (size_t)grid * kScalarTile * (head_dim + 2) * sizeof(float);
+    const int grid = tree_grid_of(false, n_heads, n_kv, nodes, slots);
+    const int grid_tc = head_dim == 256 ? tree_grid_of(true, n_heads, n_kv, nodes, slots) : 0;
+    if (grid < 0 || grid_tc < 0) return 0;
+    const size_t rows = (size_t)grid * kTreeScalarRows, rows_tc = (size_t)grid_tc * kTreeTcRows;
+    return (rows > rows_tc ? rows : rows_tc) * (head_dim + 2) * sizeof(float);
 }
 
 int hipml_attn_tree(hipml_stream_t stream, int kv_dtype, const int *pos, const int *parents, const float *q,
@@ -964,11 +971,13 @@ int hipml_attn_tree(hipml_stream_t stream, int kv_dtype, const int *pos, const i
     p.kv_dtype = kv_dtype;
     p.scale_log2 = scale * kLog2e;
     p.slot_bytes = kv_slot_bytes;
-    p.tile_rows = kScalarTile;
-    p.grid = tree_grid(n_heads, n_kv, nodes, slots, kScalarTile, 2 * device_sms());
+    const size_t align = reinterpret_cast<size_t>(k_cache) | reinterpret_cast<size_t>(v_cache) | (slots > 1 ? kv_slot_bytes : 0);
+    const bool tensor_core = head_dim == 256 && (align & 15) == 0;
+    p.tile_rows = tensor_core ? kTreeTcRows : kTreeScalarRows;
+    p.grid = tree_grid_of(tensor_core, n_heads, n_kv, nodes, slots);
     p.part_acc = (float *)workspace;
     p.part_ml = p.part_acc + (size_t)p.grid * p.tile_rows * head_dim;
-    if (int e = launch_tree_scalar(as_stream(stream), p)) return e;
+    if (int e = (tensor_core ? launch_tree_tc : launch_tree_scalar)(as_stream(stream), p)) return e;
     return launch_tree_fold(as_stream(stream), p);
 }
 

@@ -153,6 +153,10 @@ __device__ __forceinline__ void tree_ancestors(const int *parents, int node, uns
 
 // attn_tree.cu: the CUDA-core kernel (any head size and alignment) and the fold of the runs.
 int launch_tree_scalar(cudaStream_t stream, const TreeParams &p);
+constexpr int kTreeScalarRows = 32;
+// attn_tree_tc.cu: head_dim 256, caches (and slots) on 16 bytes.
+int launch_tree_tc(cudaStream_t stream, const TreeParams &p);
+constexpr int kTreeTcRows = 128;
 int launch_tree_fold(cudaStream_t stream, const TreeParams &p);
 
 // tree_verify.cu
