@@ -62,7 +62,7 @@ __global__ void __launch_bounds__(256) attn_tree_scalar(TreeParams p) {
     griddep_wait();
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     if (warp == 0) {
-        const TreeItem it = tree_item(p, tree_quota(p), blockIdx.x);
+        const TreeItem it = tree_item(p, blockIdx.x);
         if (lane == 0) s_item = it;
     }
     __syncthreads();
@@ -84,10 +84,7 @@ __global__ void __launch_bounds__(256) attn_tree_scalar(TreeParams p) {
     }
     __syncthreads();
     if (tid < rows) {
-        unsigned words[kTreeWords];
-        tree_ancestors(s_parents, (it.tile * kRows + tid) / p.group, words, p.status);
-#pragma unroll
-        for (int w = 0; w < kTreeWords; w++) s_sees[tid][w] = words[w];
+        tree_ancestors(s_parents, (it.tile * kRows + tid) / p.group, s_sees[tid], p.status);
     }
     const unsigned char *const kc = p.k + (size_t)it.slot * p.slot_bytes, *const vc = p.v + (size_t)it.slot * p.slot_bytes;
     float acc[kWarpRows][kB], m[kWarpRows], l[kWarpRows];
@@ -172,74 +169,84 @@ __global__ void __launch_bounds__(256) attn_tree_scalar(TreeParams p) {
     }
 }
 
-// The runs of a query row, folded: grid (n_heads * nodes, slots), 256 threads; a column of four dims has 1024 / head_dim
-// threads, which take the runs in turn.
+// The runs of a query row, folded: grid (n_heads * nodes, slots), 256 threads. A column of four dims has 1024 / head_dim
+// threads, which take the runs in turn, relative to a maximum of their own (so that a run's row and its pair are one trip
+// to memory, after that for the slot's share), and meet in shared memory.
 __global__ void __launch_bounds__(256) attn_tree_fold(TreeParams p) {
-    __shared__ int s_quota, s_first;
-    __shared__ float s_max[8];
+    __shared__ float s_max[256], s_den[256];
     __shared__ float4 s_sum[256];
-    __shared__ float s_den[256];
     griddep_launch();
     griddep_wait();
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int tid = threadIdx.x;
     const int slot = blockIdx.y, node = blockIdx.x / p.n_heads, head = blockIdx.x - node * p.n_heads;
+    const int4 share = __ldcg(p.shares + slot);
     const TreeSlot t = tree_slot(p.pos, slot, p.stride, p.nodes);
-    if (node >= t.live) return;
-    if (warp == 0) {
-        const int quota = tree_quota(p);
-        int first = 0;
-        for (int s = lane; s < slot; s += 32) first += tree_ctas(p, tree_slot(p.pos, s, p.stride, p.nodes), quota);
-        first = __reduce_add_sync(0xffffffffu, first);
-        if (lane == 0) {
-            s_quota = quota;
-            s_first = first;
-        }
-    }
-    __syncthreads();
-    const int runs = div_up_int(t.base + t.live, kTreeKeyTile * s_quota);
-    if (runs == 1) return;   // (written by the run itself)
+    const int runs = share.y;
+    if (node >= t.live || runs == 1) return;   // (one run has written the row itself)
     const int kvh = head / p.group, at = node * p.group + head - kvh * p.group;
     const int tile = at / p.tile_rows, r = at - tile * p.tile_rows;
-    const int tiles = div_up_int(t.live * p.group, p.tile_rows);
-    const size_t first = (size_t)s_first + (size_t)(kvh * tiles + tile) * runs;
-    const float2 *const ml = reinterpret_cast<const float2 *>(p.part_ml) + first * p.tile_rows + r;
-    float big = -INFINITY;
-    for (int j = tid; j < runs; j += 256) big = fmaxf(big, ml[(size_t)j * p.tile_rows].x);
-    big = warp_max(big);
-    if (lane == 0) s_max[warp] = big;
-    __syncthreads();
-#pragma unroll
-    for (int w = 0; w < 8; w++) big = fmaxf(big, s_max[w]);
+    const size_t first = (size_t)share.x + (size_t)(kvh * share.z + tile) * runs;
     const int cols = p.head_dim / 4, groups = 256 / cols;
     const int col = tid % cols, g = tid / cols;
     float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    float den = 0.0f;
+    float den = 0.0f, big = -INFINITY;
     if (g < groups) {
+        const float2 *const ml = reinterpret_cast<const float2 *>(p.part_ml) + first * p.tile_rows + r;
         const float4 *const acc = reinterpret_cast<const float4 *>(p.part_acc + (first * p.tile_rows + r) * p.head_dim) + col;
         const size_t step = (size_t)p.tile_rows * cols;
-#pragma unroll 4
-        for (int j = g; j < runs; j += groups) {
-            const float2 x = ml[(size_t)j * p.tile_rows];
-            const float4 a = acc[j * step];
-            const float w = x.x == -INFINITY ? 0.0f : exp2f(x.x - big);   // (a run of which the row sees nothing)
-            sum.x = fmaf(a.x, w, sum.x);
-            sum.y = fmaf(a.y, w, sum.y);
-            sum.z = fmaf(a.z, w, sum.z);
-            sum.w = fmaf(a.w, w, sum.w);
-            den = fmaf(x.y, w, den);
+        constexpr int kAtOnce = 5;
+        for (int j0 = g; j0 < runs; j0 += groups * kAtOnce) {
+            float2 x[kAtOnce];
+            float4 a[kAtOnce];
+            float most = big;
+#pragma unroll
+            for (int k = 0; k < kAtOnce; k++) {
+                const int j = j0 + k * groups;
+                x[k] = make_float2(-INFINITY, 0.0f);
+                if (j < runs) {
+                    x[k] = __ldcg(ml + (size_t)j * p.tile_rows);
+                    a[k] = __ldcg(acc + (size_t)j * step);
+                }
+            }
+#pragma unroll
+            for (int k = 0; k < kAtOnce; k++) most = fmaxf(most, x[k].x);
+            const float corr = big == -INFINITY ? 0.0f : exp2f(big - most);
+            sum.x *= corr;
+            sum.y *= corr;
+            sum.z *= corr;
+            sum.w *= corr;
+            den *= corr;
+            big = most;
+#pragma unroll
+            for (int k = 0; k < kAtOnce; k++) {
+                if (x[k].x == -INFINITY) continue;   // (no run, or one of which the row sees nothing)
+                const float w = exp2f(x[k].x - big);
+                sum.x = fmaf(a[k].x, w, sum.x);
+                sum.y = fmaf(a[k].y, w, sum.y);
+                sum.z = fmaf(a[k].z, w, sum.z);
+                sum.w = fmaf(a[k].w, w, sum.w);
+                den = fmaf(x[k].y, w, den);
+            }
         }
     }
+    s_max[tid] = big;
     s_sum[tid] = sum;
     s_den[tid] = den;
     __syncthreads();
     if (g == 0) {
-        for (int i = 1; i < groups; i++) {
+        for (int i = 1; i < groups; i++) big = fmaxf(big, s_max[i * cols + col]);
+        sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        den = 0.0f;
+        for (int i = 0; i < groups; i++) {
+            const float m = s_max[i * cols + col];
+            if (m == -INFINITY) continue;
+            const float w = exp2f(m - big);
             const float4 a = s_sum[i * cols + col];
-            sum.x += a.x;
-            sum.y += a.y;
-            sum.z += a.z;
-            sum.w += a.w;
-            den += s_den[i * cols + col];
+            sum.x = fmaf(a.x, w, sum.x);
+            sum.y = fmaf(a.y, w, sum.y);
+            sum.z = fmaf(a.z, w, sum.z);
+            sum.w = fmaf(a.w, w, sum.w);
+            den = fmaf(s_den[i * cols + col], w, den);
         }
         const float inv = 1.0f / den;
         reinterpret_cast<float4 *>(p.out + (((size_t)slot * p.nodes + node) * p.n_heads + head) * p.head_dim)[col] =

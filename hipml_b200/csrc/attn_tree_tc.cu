@@ -27,7 +27,9 @@
 // Sums: the tensor cores cut their f32 accumulators off instead of rounding them, 3.5e-9 relative per key of an unbroken
 // chain, so every kFlushKeys keys O leaves TMEM for the run's partial in memory (added there, in f32).
 //
-// Warps 0-7 softmax and epilogue, 8-15 planes, 16 copies, 17 MMAs. Waits are bounded: one that runs out sets the device
+// Warps 0-7 softmax and epilogue, 8-11 planes of K, 12-15 of V, 16 copies, 17 MMAs (the whole warp runs that loop and one
+// elected lane issues: from a branch of a single lane every descriptor went through a move to the uniform registers, 46
+// cycles an MMA of N = 64 and 83 beside the other warps, against 32), 18 the factors of V's rows. Waits are bounded: one that runs out sets the device
 // status and a flag that turns every other wait of the CTA into none; all warps still come to every barrier, nothing is
 // written out, and copies and MMAs in flight are waited for (bounded too) before shared memory and TMEM are released.
 #include <atomic>
@@ -43,32 +45,36 @@ namespace {
 using namespace ptx;
 
 constexpr int kD = 256, kRows = kTreeTcRows;
-constexpr int kThreads = 18 * 32;
-constexpr int kPlaneThreads = 256;
+constexpr int kThreads = 19 * 32;
+constexpr int kGroup = 4;                        // warps that make planes: four of K, four of V
 constexpr int kQChunk = kRows * 128;             // 128 rows x 64 dims, f16
 constexpr int kQBytes = 4 * kQChunk;             // one plane of Q
-constexpr int kStages = 3, kStageBytes = 32 * 1024;
+constexpr int kStages = 2;                       // of K and of V
+constexpr int kKStage = 32 * 1024, kVStage = 16 * 1024;
 constexpr int kRawBytes = 3 * 64 * 272;
 constexpr int kFlushKeys = 1024;
 constexpr unsigned kSpinLimit = 1u << 22;
 constexpr float kThreshold = 8.0f;               // log2: the reference moves when a weight would exceed 2^8 times it,
 constexpr float kLift = 7.0f;                    // and weights are kept 2^7 times larger: below 2^15, f16's smallest 2^-24
-constexpr float kLeastPower = -100.0f;           // of a value row; smaller values count as 0 (as do rows of zeros)
+constexpr int kLeastPower = -100, kMostPower = 100;   // of a key or value row; smaller values count as 0 (as do rows of zeros)
 
 template <int kType>   // 0 f32, 1 q8_0, 2 q4_0
 struct Shape {
     static constexpr int kKeys = kType == 0 ? 32 : 64;         // of a tile
-    static constexpr int kParts = kType == 0 ? 1 : 2;          // stages of a K (or V) tile, by dims
-    static constexpr int kChunks = 4 / kParts;                 // of 64 dims, in a stage
+    static constexpr int kParts = kType == 0 ? 1 : 2;          // of a row, by dims
+    static constexpr int kChunks = 4 / kParts;                 // of 64 dims, in a part
+    // a stage of K has a part of a tile's rows, one of V a part of half of them; hi plane, then lo
     static constexpr int kChunkBytes = kKeys * 128;
-    static constexpr int kPlaneBytes = kChunks * kChunkBytes;  // hi, then lo
-    static_assert(2 * kPlaneBytes == kStageBytes, "a stage is two planes");
-    // the raw ring: f32 in pieces of 16 rows, padded apart so that eight rows' 16-byte words fall into different banks
+    static constexpr int kPlaneBytes = kChunks * kChunkBytes;
+    static constexpr int kVKeys = kKeys / 2;
+    static constexpr int kVChunkBytes = kVKeys * 128;
+    static constexpr int kVPlaneBytes = kChunks * kVChunkBytes;
+    static_assert(2 * kPlaneBytes == kKStage && 2 * kVPlaneBytes == kVStage, "a stage is two planes");
+    // the raw ring has half tiles (f32 rows padded apart so that eight rows' 16-byte words fall into different banks)
     static constexpr int kRowPitch = kType == 0 ? 1040 : (kType == 1 ? 272 : 144);
-    static constexpr int kRawRows = kType == 0 ? 16 : 64;
+    static constexpr int kRawRows = kKeys / 2;
     static constexpr int kRawSlot = kRawRows * kRowPitch;
-    static constexpr int kRawSlots = kRawBytes / kRawSlot;
-    static constexpr int kPieces = kKeys / kRawRows;           // raw slots of a tile
+    static constexpr int kRawSlots = kRawBytes / kRawSlot < 8 ? kRawBytes / kRawSlot : 8;
     static constexpr int kHalf = kKeys / 2;                    // keys of a softmax thread
     // the 32 dims that make block b of part h of a row. Quantised blocks come in pairs (an odd block begins inside a word):
     // a part has one block of each pair, so that eight rows' four pairs fall into different banks.
@@ -76,21 +82,29 @@ struct Shape {
 };
 
 constexpr int kOffQ = 0;                                   // Q lo
-constexpr int kOffStages = kOffQ + kQBytes;
-constexpr int kOffRaw = kOffStages + kStages * kStageBytes;
-constexpr int kOffKey = kOffRaw + kRawBytes;               // [3][64] factor of S, by key
-constexpr int kOffPow = kOffKey + 3 * 64 * 4;              // [2][64] E
-constexpr int kOffInv = kOffPow + 2 * 64 * 4;              // [2][64] 2^-E
-constexpr int kOffMeet = kOffInv + 2 * 64 * 4;             // [2][2][128]: the halves of a row meet
+constexpr int kOffK = kOffQ + kQBytes;
+constexpr int kOffV = kOffK + kStages * kKStage;
+constexpr int kOffRaw = kOffV + kStages * kVStage;
+// A tile's factors of K are written once its planes have their stage, those of V once its rows are in the ring. By then the
+// tile four before has been through the softmax: W V of tile t - 4 was issued before Q K^T of t - 2, which had to be done
+// for the stage to be free, and the slot of the ring that V's rows take was free at the earliest when planes were made that
+// needed the same.
+constexpr int kFactors = 4;
+constexpr int kOffKey = kOffRaw + kRawBytes;               // [kFactors][64] factor of S, by key
+constexpr int kOffPow = kOffKey + kFactors * 64 * 4;       // [kFactors][64] E
+constexpr int kOffInv = kOffPow + kFactors * 64 * 4;       // [kFactors][64] 2^-E
+constexpr int kOffMeet = kOffInv + kFactors * 64 * 4;      // [2][2][128]: the halves of a row meet
 constexpr int kOffRowFac = kOffMeet + 2 * 2 * 128 * 4;     // [128]
 constexpr int kOffSees = kOffRowFac + kRows * 4;           // [128][kTreeWords + 1]
 constexpr int kOffParents = kOffSees + kRows * (kTreeWords + 1) * 4;
 constexpr int kOffBars = kOffParents + kTreeNodes * 4;
-constexpr int kSmemNeed = kOffBars + 256;
-constexpr int kSmemBytes = kSmemNeed + 1024;               // (the planes lie on 1 KB boundaries)
+constexpr int kBars = 43;
+constexpr int kSmemNeed = kOffBars + kBars * 8;
+constexpr int kSmemBytes = (kSmemNeed + 15) / 16 * 16 + 1024;               // (the planes lie on 1 KB boundaries)
 static_assert(kSmemBytes <= 227 * 1024, "one CTA per SM");
 constexpr int kOutPitch = kD + 4;                          // floats of a staged output row
 static_assert(kRows * kOutPitch * 4 <= kOffRaw, "the output rows are staged over Q and the planes");
+static_assert(kQBytes <= kStages * kKStage, "Q hi passes through K's stages");
 
 constexpr unsigned kTmemO = 0, kTmemS = 256, kTmemQ = 384;   // columns; S: two tiles of 64
 
@@ -99,17 +113,31 @@ __device__ __forceinline__ unsigned desc_lo_mn(unsigned addr, unsigned pitch) {
     return ((addr & 0x3ffff) >> 4) | (pitch >> 4) << 16;
 }
 
+// The kernel's code is kept small: its roles together, and what runs once, come through one instruction cache (with every
+// loop unrolled a tile of 64 rows took 10,000 cycles and Q 6,700). Loops over blocks, rows and chunks are loops.
+__device__ __noinline__ void wait_long(unsigned bar, unsigned parity, volatile int *abort, int *status, int code) {
+    for (unsigned i = 0; i < kSpinLimit; i++) {
+        if (mbar_try_wait(bar, parity)) return;
+        if ((i & 255) == 255 && *abort) return;
+        if (i > 4096) __nanosleep(64);
+    }
+    atomicCAS(status, 0, code);
+    *abort = 1;
+}
+__device__ __forceinline__ bool elect_one() {
+    unsigned p;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "elect.sync _|p, 0xffffffff;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(p));
+    return p != 0;
+}
 struct Waits {
     volatile int *abort;
     int *status;
     __device__ __forceinline__ void operator()(unsigned bar, unsigned parity, int code) const {
-        for (unsigned i = 0; i < kSpinLimit; i++) {
-            if (mbar_try_wait(bar, parity)) return;
-            if ((i & 255) == 255 && *abort) return;
-            if (i > 4096) __nanosleep(64);
-        }
-        atomicCAS(status, 0, code);
-        *abort = 1;
+        if (!mbar_try_wait(bar, parity)) wait_long(bar, parity, abort, status, code);
     }
 };
 
@@ -132,30 +160,75 @@ __device__ __forceinline__ void split_pair(float a, float b, unsigned &hi, unsig
 // 2^n for whole n of [-126, 127]
 __device__ __forceinline__ float power(int n) { return __int_as_float((n + 127) << 23); }
 
-// A quantised block's 32 values (scale `s` in range), as hi and lo words in the order of the dims.
+// The power of two that brings a row into range, from its largest |value| (f32: its bits) or |scale| (its bits): values come
+// to [2^10, 2^11), scales to [8, 16), so that codes times them stay below 2^11 and lo is exact.
 template <int kType>
-__device__ __forceinline__ void block_planes(const unsigned *w, bool odd, __half2 s, unsigned (&hi)[16], unsigned (&lo)[16]) {
-    if constexpr (kType == 1) {
-        // even: codes in bytes 2 .. 33 of w; odd: in whole words from 1 on (word 0 holds the scale)
-#pragma unroll
-        for (int j = 0; j < 8; j++) {
-            const unsigned c = (odd ? w[1 + j] : __byte_perm(w[j], w[j + 1], 0x5432)) ^ 0x80808080u;
-            // 0x6400 | byte is 1024 + byte
-            const __half2 bias = __float2half2_rn(1152.0f);
-            const __half2 a = __hsub2(as_half2(__byte_perm(c, 0x64646464u, 0x4140)), bias);
-            const __half2 b = __hsub2(as_half2(__byte_perm(c, 0x64646464u, 0x4342)), bias);
-            split_product(a, s, hi[2 * j], lo[2 * j]);
-            split_product(b, s, hi[2 * j + 1], lo[2 * j + 1]);
+__device__ __forceinline__ int row_power(unsigned most, bool &bad) {
+    bad = most >= (kType == 0 ? 0x7f800000u : 0x7c00u);
+    if (bad) return 0;
+    if (kType == 0) return min(max((int)(most >> 23) - 127 - 10, kLeastPower), kMostPower);
+    return most == 0 ? kLeastPower : max((int)most >> 10, 1) - 15 - 3;
+}
+// The largest |value| of half of an f32 row, or |scale| of a quantised row, as bits.
+template <int kType>
+__device__ __forceinline__ unsigned row_most(const unsigned char *row, int half) {
+    unsigned most = 0;
+    if constexpr (kType == 0) {
+#pragma unroll 4
+        for (int k = 0; k < 32; k++) {
+            const uint4 x = reinterpret_cast<const uint4 *>(row)[32 * half + k];
+            most = max(max(most, x.x & 0x7fffffffu), max(max(x.y & 0x7fffffffu, x.z & 0x7fffffffu), x.w & 0x7fffffffu));
         }
     } else {
 #pragma unroll
-        for (int j = 0; j < 4; j++) {
-            const unsigned c = odd ? w[1 + j] : __byte_perm(w[j], w[j + 1], 0x5432);
-            const __half2 bias = __float2half2_rn(1032.0f);
-            const unsigned even = __byte_perm(c, 0, 0x4140), next = __byte_perm(c, 0, 0x4342);   // bytes 0, 1 and 2, 3
+        for (int b = 0; b < 8; b++)
+            most = max(most, (unsigned)(*reinterpret_cast<const unsigned short *>(row + b * (kType == 1 ? 34 : 18)) & 0x7fff));
+    }
+    return most;
+}
+
+// The power of two of a value row in shared memory, clamped: by a whole warp.
+template <int kType>
+__device__ __forceinline__ int first_power(const unsigned char *row, int lane) {
+    int top;
+    if constexpr (kType == 0) {
+        const uint4 *const src = reinterpret_cast<const uint4 *>(row) + 2 * lane;
+        unsigned most = 0;
 #pragma unroll
-            for (int e = 0; e < 2; e++) {
-                const unsigned x = e ? next : even;
+        for (int k = 0; k < 2; k++) {
+            const uint4 x = src[k];
+            most = max(max(most, x.x & 0x7fffffffu), max(max(x.y & 0x7fffffffu, x.z & 0x7fffffffu), x.w & 0x7fffffffu));
+        }
+        most = __reduce_max_sync(0xffffffffu, most);
+        top = most > 0 ? (int)(most >> 23) - 127 - 10 : 0;
+    } else {
+        const unsigned short scale = *reinterpret_cast<const unsigned short *>(row + (lane & 7) * (kType == 1 ? 34 : 18));
+        const int most = __reduce_max_sync(0xffffffffu, (int)(scale & 0x7fff));
+        top = most > 0 ? max(most >> 10, 1) - 15 - 3 : 0;
+    }
+    return min(max(top, -20), 16);
+}
+
+// A quantised block's 32 values times scale, as hi and lo words in the order of the dims. `w`: its words from the one that
+// holds its scale on. An even block's codes begin in the middle of that word (take = 0x5432), an odd one's behind it (0x7654).
+template <int kType>
+__device__ __forceinline__ void block_planes(const unsigned *w, unsigned take, __half2 s, unsigned (&hi)[16], unsigned (&lo)[16]) {
+    if constexpr (kType == 1) {
+        const __half2 bias = __float2half2_rn(1152.0f);   // 0x6400 | byte is 1024 + byte
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+            const unsigned c = __byte_perm(w[j], w[j + 1], take) ^ 0x80808080u;
+            split_product(__hsub2(as_half2(__byte_perm(c, 0x64646464u, 0x4140)), bias), s, hi[2 * j], lo[2 * j]);
+            split_product(__hsub2(as_half2(__byte_perm(c, 0x64646464u, 0x4342)), bias), s, hi[2 * j + 1], lo[2 * j + 1]);
+        }
+    } else {
+        const __half2 bias = __float2half2_rn(1032.0f);
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            const unsigned c = __byte_perm(w[j], w[j + 1], take);
+#pragma unroll
+            for (int e = 0; e < 2; e++) {   // bytes 0, 1 and 2, 3; the low nibbles are values j, the high ones j + 16
+                const unsigned x = __byte_perm(c, 0, e ? 0x4342 : 0x4140);
                 split_product(__hsub2(as_half2((x & 0x000f000fu) | 0x64006400u), bias), s, hi[2 * j + e], lo[2 * j + e]);
                 split_product(__hsub2(as_half2(((x >> 4) & 0x000f000fu) | 0x64006400u), bias), s, hi[8 + 2 * j + e],
                               lo[8 + 2 * j + e]);
@@ -172,30 +245,35 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tree_tc(TreeParams p) {
     unsigned char *const smem =
         reinterpret_cast<unsigned char *>((reinterpret_cast<size_t>(smem_raw) + 1023) & ~(size_t)1023);
     __shared__ TreeItem s_item;
-    __shared__ int s_abort;
+    __shared__ int s_abort, s_power0;
     __shared__ unsigned s_tmem;
     griddep_launch();
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     uint64_t *const bars = reinterpret_cast<uint64_t *>(smem + kOffBars);
-    const unsigned raw_full = smem_u32(bars), raw_empty = smem_u32(bars + 5), st_full = smem_u32(bars + 10),
-                   st_empty = smem_u32(bars + 13), s_ready = smem_u32(bars + 16), w_ready = smem_u32(bars + 18),
-                   o_done = smem_u32(bars + 20), factors = smem_u32(bars + 22), all_done = smem_u32(bars + 24);
-    static_assert(T::kRawSlots <= 5, "raw barriers");
+    // raw rows: full by the half tile's number, eight of K and eight of V (whoever waits for one waits for all of its kind, in
+    // their order, so no phase is taken for another), empty by the slot
+    const unsigned raw_full = smem_u32(bars), raw_empty = smem_u32(bars + 16), k_full = smem_u32(bars + 24),
+                   k_empty = smem_u32(bars + 26), v_full = smem_u32(bars + 28), v_empty = smem_u32(bars + 30),
+                   s_ready = smem_u32(bars + 32), w_ready = smem_u32(bars + 34), o_done = smem_u32(bars + 36),
+                   factors = smem_u32(bars + 38), all_done = smem_u32(bars + 42);
+    static_assert(T::kRawSlots <= 8 && kFactors <= 4 && kBars == 43, "barriers");
+    auto raw_bar = [&](bool v, int i) { return raw_full + 8 * ((v ? 8 : 0) + (i & 7)); };   // of half tile i
     if (tid == 0) {
+        for (int i = 0; i < 16; i++) mbar_init(raw_full + 8 * i, 1);
         for (int i = 0; i < T::kRawSlots; i++) {
-            mbar_init(raw_full + 8 * i, 1);
-            mbar_init(raw_empty + 8 * i, kPlaneThreads / 32 / T::kPieces);   // the warps that read the slot
-        }
-        for (int i = 0; i < kStages; i++) {
-            mbar_init(st_full + 8 * i, kPlaneThreads / 32);
-            mbar_init(st_empty + 8 * i, 1);
+            // four warps make planes of a slot's rows; warp 18 reads V's as well (and K's first warp arrives once more)
+            mbar_init(raw_empty + 8 * i, kGroup + 1);
         }
         for (int i = 0; i < 2; i++) {
+            mbar_init(k_full + 8 * i, kGroup);
+            mbar_init(k_empty + 8 * i, 1);
+            mbar_init(v_full + 8 * i, kGroup);
+            mbar_init(v_empty + 8 * i, 1);
             mbar_init(s_ready + 8 * i, 1);
             mbar_init(w_ready + 8 * i, 8);
             mbar_init(o_done + 8 * i, 1);
-            mbar_init(factors + 8 * i, kPlaneThreads / 32);
         }
+        for (int i = 0; i < kFactors; i++) mbar_init(factors + 8 * i, kGroup + 1);
         mbar_init(all_done, 1);
         s_abort = 0;
         mbar_init_fence();
@@ -204,7 +282,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tree_tc(TreeParams p) {
     tc_fence_before();
     griddep_wait();
     if (warp == 0) {
-        const TreeItem it = tree_item(p, tree_quota(p), blockIdx.x);
+        const TreeItem it = tree_item(p, blockIdx.x);
         if (lane == 0) s_item = it;
     }
     __syncthreads();
@@ -220,30 +298,29 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tree_tc(TreeParams p) {
         const int at = it.tile * kRows + r, node = at / p.group;
         return (first_node + node) * p.n_heads + it.kvh * p.group + (at - node * p.group);
     };
-    // The tiles' K and V in the order in which the MMAs take them: K0 K1 V0 K2 V1 ... V(n-1).
-    const int units = 2 * n;
-    auto unit_is_v = [&](int m) { return n == 1 ? m == 1 : (m >= 2 && (m & 1) == 0) || m == units - 1; };
-    auto unit_tile = [&](int m) {
-        if (m == units - 1) return n - 1;
-        return m == 0 ? 0 : ((m & 1) ? (m + 1) / 2 : (m - 2) / 2);
-    };
+    // Half tiles in the raw ring: K0 K1 V0 K2 V1 .. V(n-1). A slot of V is free when its planes are made, in the middle of
+    // its W V, and what takes it is then K of two tiles later. (K0 V0 K1 V1: K of the next tile, whose copy everything waited
+    // for.)
+    auto raw_of = [&](bool v, int t) { return v ? (t == n - 1 ? 4 * t + 2 : 4 * t + 4) : (t == 0 ? 0 : 4 * t - 2); };
     const size_t slot_at = (size_t)it.slot * p.slot_bytes;
     auto tile_rows = [&](int t) { return min(T::kKeys, hi_key - (lo_key + t * T::kKeys)); };
 
     if (warp == 16 && n > 0) {
         // ------------------------------------------------------------ copies
-        unsigned c = 0;   // raw slots filled
-        for (int m = 0; m < units && !*wait.abort; m++) {
-            const int t = unit_tile(m), live = tile_rows(t);
-            const unsigned char *const cache = (unit_is_v(m) ? p.v : p.k) + slot_at;
-            for (int piece = 0; piece < T::kPieces; piece++, c++) {
+        unsigned c = 0, c_k = 0, c_v = 0;   // half tiles asked for, of K, of V
+        for (int m = 0; m < 2 * n && !*wait.abort; m++) {
+            const bool is_v = m == 2 * n - 1 || (m > 0 && (m & 1) == 0);
+            const int t = m == 2 * n - 1 ? n - 1 : (is_v ? m / 2 - 1 : (m + 1) / 2), live = tile_rows(t);
+            const unsigned char *const cache = (is_v ? p.v : p.k) + slot_at;
+            for (int piece = 0; piece < 2; piece++, c++) {
                 const unsigned slot = c % T::kRawSlots, round = c / T::kRawSlots;
                 wait(raw_empty + 8 * slot, (round & 1) ^ 1, 51);
                 const int key = lo_key + t * T::kKeys + piece * T::kRawRows;
                 const int here = min(max(live - piece * T::kRawRows, 0), T::kRawRows);
-                const unsigned dst = smem_u32(smem + kOffRaw) + slot * T::kRawSlot, bar = raw_full + 8 * slot;
+                const unsigned dst = smem_u32(smem + kOffRaw) + slot * T::kRawSlot, bar = raw_bar(is_v, 2 * t + piece);
                 const bool go = !*wait.abort;
                 if (__any_sync(0xffffffffu, !go)) break;
+                (is_v ? c_v : c_k)++;
                 if constexpr (kType == 0) {
                     if (lane == 0) mbar_arrive_expect_tx(bar, here * kD * 4);
                     __syncwarp();
@@ -258,295 +335,353 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tree_tc(TreeParams p) {
         }
         __syncwarp();
         if (*wait.abort) {
-            // what is on its way lands before shared memory is released
-            for (unsigned i = c > (unsigned)T::kRawSlots ? c - T::kRawSlots : 0; i < c; i++)
-                for (unsigned spin = 0; spin < kSpinLimit; spin++)
-                    if (mbar_try_wait(raw_full + 8 * (i % T::kRawSlots), (i / T::kRawSlots) & 1)) break;
+            // what is on its way lands before shared memory is released: the last half tiles of both kinds
+            for (int i = 0; i < 16; i++) {
+                const unsigned used = i < 8 ? c_k : c_v;   // half tiles asked for
+                const unsigned last = used > (unsigned)(i & 7) ? (used - 1 - (i & 7)) / 8 : 0;   // uses of the barrier, less one
+                if (used > (unsigned)(i & 7))
+                    for (unsigned spin = 0; spin < kSpinLimit; spin++)
+                        if (mbar_try_wait(raw_full + 8 * i, last & 1)) break;
+            }
         }
     }
 
-    if (warp < 16 && n > 0) {
-        // ------------------------------------------------------------ Q: eight rows a warp
-        float4 x[8][2];
-#pragma unroll
-        for (int j = 0; j < 8; j++) {
-            const int r = warp * 8 + j;
-            x[j][0] = x[j][1] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-            if (r < rows) {
-                const float4 *const src = reinterpret_cast<const float4 *>(p.q + head_row(r) * kD) + 2 * lane;
-                x[j][0] = __ldg(src);
-                x[j][1] = __ldg(src + 1);
-            }
-        }
-        for (int i = tid; i < it.live; i += 512)
+    // ---------------------------------------------------------------- Q: warps 0-7 and 12-15, a row at a time
+    // hi goes to TMEM by way of K's stages.
+    if ((warp < 8 || (warp >= 12 && warp < 16)) && n > 0) {
+        constexpr int kQWarps = 12;
+        const int qw = warp < 8 ? warp : warp - 4;
+        // Position of dims 8 * lane .. in the order of the parts: block b of part h stands at 128 h + 32 b (f32: 32 b)
+        const int blk = lane >> 2;
+        const int at = kType == 0 ? 8 * lane : 128 * (blk & 1) + 32 * (blk >> 1) + 8 * (lane & 3);
+        unsigned char *const to = smem + kOffQ + (at >> 6) * kQChunk;
+        for (int i = tid < 256 ? tid : tid - 128; i < it.live; i += 384)
             reinterpret_cast<int *>(smem + kOffParents)[i] = p.parents[first_node + i];
+        if (tid >= rows && tid < kRows) reinterpret_cast<float *>(smem + kOffRowFac)[tid] = 0.0f;
+        auto row_at = [&](int r) { return reinterpret_cast<const float4 *>(p.q + head_row(r) * kD) + 2 * lane; };
+        constexpr int kAhead = 3;   // rows on their way
+        float4 x[kAhead][2];
 #pragma unroll
-        for (int j = 0; j < 8; j++) {
-            const int r = warp * 8 + j;
-            const float v[8] = {x[j][0].x, x[j][0].y, x[j][0].z, x[j][0].w, x[j][1].x, x[j][1].y, x[j][1].z, x[j][1].w};
-            float most = 0.0f;
-            bool bad = false;
-#pragma unroll
-            for (int e = 0; e < 8; e++) {
-                most = fmaxf(most, fabsf(v[e]));
-                bad = bad || !(fabsf(v[e]) < INFINITY);
-            }
-            most = warp_max(most);
-            bad = __any_sync(0xffffffffu, bad);
-            // the row's largest value comes to [2^10, 2^11)
-            const int e = bad ? 0 : min(max(((__float_as_int(most) >> 23) & 255) - 127 - 10, -116), 116);
-            const float f = power(-e);
-            if (lane == 0)
-                reinterpret_cast<float *>(smem + kOffRowFac)[r] =
-                    bad ? __int_as_float(0x7fffffff) : power(e) * p.scale_log2;
-            unsigned h[4], l[4];
-#pragma unroll
-            for (int k = 0; k < 4; k++) split_pair(bad ? 0.0f : v[2 * k] * f, bad ? 0.0f : v[2 * k + 1] * f, h[k], l[k]);
-            // Position of dims 8 * lane .. in the order of the parts: block b of part h stands at 128 h + 32 b (f32: 32 b)
-            const int blk = lane >> 2;
-            const int at = kType == 0 ? 8 * lane : 128 * (blk & 1) + 32 * (blk >> 1) + 8 * (lane & 3);
-            const int off = (at >> 6) * kQChunk + sw128_offset(r, at & 63);
-            *reinterpret_cast<uint4 *>(smem + kOffQ + off) = make_uint4(l[0], l[1], l[2], l[3]);
-            // (hi goes to TMEM by way of the first stages)
-            *reinterpret_cast<uint4 *>(smem + kOffStages + off) = make_uint4(h[0], h[1], h[2], h[3]);
+        for (int k = 0; k < kAhead; k++) {
+            const float4 *const src = row_at(min(qw + kQWarps * k, rows - 1));
+            x[k][0] = __ldg(src);
+            x[k][1] = __ldg(src + 1);
         }
-        named_sync(1, 512);
-        if (warp < 8) {
-            // thread (row, half) takes half of the row's hi plane to TMEM
-            const int r = tid & 127, half = tid >> 7;
-            const unsigned to = s_tmem + kTmemQ + 64 * half + ((unsigned)((warp & 3) * 32) << 16);
+#pragma unroll 1
+        for (int r = qw; r < rows; r += kQWarps) {
+            const float v[8] = {x[0][0].x, x[0][0].y, x[0][0].z, x[0][0].w, x[0][1].x, x[0][1].y, x[0][1].z, x[0][1].w};
 #pragma unroll
-            for (int c = 0; c < 2; c++) {
+            for (int k = 0; k + 1 < kAhead; k++) {
+                x[k][0] = x[k + 1][0];
+                x[k][1] = x[k + 1][1];
+            }
+            if (r + kQWarps * kAhead < rows) {
+                const float4 *const src = row_at(r + kQWarps * kAhead);
+                x[kAhead - 1][0] = __ldg(src);
+                x[kAhead - 1][1] = __ldg(src + 1);
+            }
+            unsigned most = 0;
+#pragma unroll
+            for (int e = 0; e < 8; e++) most = max(most, __float_as_uint(v[e]) & 0x7fffffffu);
+            most = __reduce_max_sync(0xffffffffu, most);
+            const bool bad = most >= 0x7f800000u;
+            // the row's largest value comes to [2^10, 2^11)
+            const int e = min(max((int)(most >> 23) - 127 - 10, -116), 116);
+            const float f = power(-e);
+            unsigned hi[4], lo[4];
+#pragma unroll
+            for (int d = 0; d < 4; d++) {
+                split_pair(v[2 * d] * f, v[2 * d + 1] * f, hi[d], lo[d]);
+                if (bad) hi[d] = lo[d] = 0;
+            }
+            if (lane == 0)
+                reinterpret_cast<float *>(smem + kOffRowFac)[r] = bad ? __int_as_float(0x7fffffff) : power(e) * p.scale_log2;
+            const int off = sw128_offset(r, at & 63);
+            *reinterpret_cast<uint4 *>(to + off) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+            *reinterpret_cast<uint4 *>(to + (kOffK - kOffQ) + off) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+        }
+        fence_async_shared();   // Q lo; the barriers below carry it on
+        named_sync(1, 32 * kQWarps);
+        if (warp < 8) {
+            // thread (row, half) takes two chunks of the row's hi plane to TMEM
+            const int r = tid & 127, half = tid >> 7;
+#pragma unroll 1
+            for (int c = 2 * half; c < 2 * half + 2; c++) {
                 unsigned q[32];
 #pragma unroll
                 for (int j = 0; j < 8; j++) {
-                    const uint4 w = *reinterpret_cast<const uint4 *>(smem + kOffStages + (2 * half + c) * kQChunk +
-                                                                     sw128_offset(r, 8 * j));
+                    const uint4 w = *reinterpret_cast<const uint4 *>(smem + kOffK + c * kQChunk + sw128_offset(r, 8 * j));
                     q[4 * j] = w.x;
                     q[4 * j + 1] = w.y;
                     q[4 * j + 2] = w.z;
                     q[4 * j + 3] = w.w;
                 }
-                tmem_st32(to + 32 * c, q);
+                tmem_st32(s_tmem + kTmemQ + 32 * c + ((unsigned)((warp & 3) * 32) << 16), q);
             }
             tmem_wait_st();
-            if (half == 0 && hi_key > it.base) {
+            named_arrive(7, 12 * 32);   // K's stages are free
+            if (tid < kRows && hi_key > it.base) {
                 // which drafted rows this row sees (rows past the last: those of the last)
-                unsigned words[kTreeWords];
-                tree_ancestors(reinterpret_cast<const int *>(smem + kOffParents), (it.tile * kRows + min(r, rows - 1)) / p.group,
-                               words, p.status);
-                unsigned *const at = reinterpret_cast<unsigned *>(smem + kOffSees) + r * (kTreeWords + 1);
-#pragma unroll
-                for (int w = 0; w < kTreeWords; w++) at[w] = words[w];
-                at[kTreeWords] = 0;
+                unsigned *const sees = reinterpret_cast<unsigned *>(smem + kOffSees) + tid * (kTreeWords + 1);
+                tree_ancestors(reinterpret_cast<const int *>(smem + kOffParents), (it.tile * kRows + min(tid, rows - 1)) / p.group,
+                               sees, p.status);
+                sees[kTreeWords] = 0;
             }
         }
-        fence_async_shared();
     }
     tc_fence_before();
-    if (warp != 16) named_sync(6, kThreads - 32);   // (the copies go on meanwhile)
+    if (warp < 8 || warp == 17) named_sync(6, 9 * 32);   // Q is there (the planes are under way meanwhile)
     tc_fence_after();
     const unsigned tmem = s_tmem;
 
     if (warp == 17) {
         // ------------------------------------------------------------ MMAs
-        if (lane == 0 && n > 0) {
+        if (n > 0) {
             constexpr unsigned kMn = 1u << 16;   // B with N contiguous
             constexpr unsigned kIdescS = idesc_f16(128, T::kKeys), kIdescO = idesc_f16(128, 64 * T::kChunks) | kMn;
-            const unsigned q_lo = desc_lo_sw128(smem_u32(smem + kOffQ)), stages = smem_u32(smem + kOffStages);
-            unsigned c = 0;   // stages consumed
-            auto stage = [&](int code) {
-                wait(st_full + 8 * (c % kStages), (c / kStages) & 1, code);
-                tc_fence_after();
-                return stages + (c % kStages) * kStageBytes;
-            };
-            auto release = [&]() {
-                tc_commit<1>(st_empty + 8 * (c % kStages));
-                c++;
-            };
+            const unsigned q_lo = desc_lo_sw128(smem_u32(smem + kOffQ));
+            unsigned vc = 0;   // stages of V consumed
+            unsigned kc = 0;   // stages of K consumed
             auto qk = [&](int i) {
                 const unsigned d = tmem + kTmemS + 64 * (i & 1);
-                for (int h = 0; h < T::kParts; h++) {
-                    const unsigned at = stage(52);
+#pragma unroll 1
+                for (int h = 0; h < T::kParts; h++, kc++) {
+                    wait(k_full + 8 * (kc % kStages), (kc / kStages) & 1, 52);
+                    __syncwarp();
                     if (*wait.abort) return;
+                    tc_fence_after();
+                    const unsigned at = smem_u32(smem + kOffK) + (kc % kStages) * kKStage;
+                    const unsigned qh = tmem + kTmemQ + 32 * T::kChunks * h, ql = q_lo + T::kChunks * h * (kQChunk >> 4);
+                    // the small terms first: each MMA cuts the sum off, relative to what it has come to
+#pragma unroll 1
+                    for (int c = 0; c < T::kChunks; c++) {
+                        const unsigned lo = desc_lo_sw128(at + T::kPlaneBytes + c * T::kChunkBytes);
+                        if (elect_one()) {
 #pragma unroll
-                    for (int ch = 0; ch < T::kChunks; ch++) {
-                        const unsigned hi = desc_lo_sw128(at + ch * T::kChunkBytes);
-                        const unsigned lo = desc_lo_sw128(at + T::kPlaneBytes + ch * T::kChunkBytes);
-                        const int chunk = h * T::kChunks + ch;
-                        const unsigned qh = tmem + kTmemQ + 32 * chunk, ql = q_lo + chunk * (kQChunk >> 4);
-#pragma unroll
-                        for (int k = 0; k < 4; k++)
-                            tc_mma_ts<1>(d, qh + 8 * k, desc_from(lo + 2 * k), kIdescS, (h | ch | k) != 0);
-#pragma unroll
-                        for (int k = 0; k < 4; k++) tc_mma_ss<1>(d, desc_from(ql + 2 * k), desc_from(hi + 2 * k), kIdescS, 1);
-#pragma unroll
-                        for (int k = 0; k < 4; k++) tc_mma_ts<1>(d, qh + 8 * k, desc_from(hi + 2 * k), kIdescS, 1);
+                            for (int k = 0; k < 4; k++)
+                                tc_mma_ts<1>(d, qh + 32 * c + 8 * k, desc_from(lo + 2 * k), kIdescS, (h | c | k) != 0);
+                        }
                     }
-                    release();
+#pragma unroll 1
+                    for (int c = 0; c < T::kChunks; c++) {
+                        const unsigned hi = desc_lo_sw128(at + c * T::kChunkBytes), q = ql + c * (kQChunk >> 4);
+                        if (elect_one()) {
+#pragma unroll
+                            for (int k = 0; k < 4; k++) tc_mma_ss<1>(d, desc_from(q + 2 * k), desc_from(hi + 2 * k), kIdescS, 1);
+                        }
+                    }
+#pragma unroll 1
+                    for (int c = 0; c < T::kChunks; c++) {
+                        const unsigned hi = desc_lo_sw128(at + c * T::kChunkBytes);
+                        if (elect_one()) {
+#pragma unroll
+                            for (int k = 0; k < 4; k++) tc_mma_ts<1>(d, qh + 32 * c + 8 * k, desc_from(hi + 2 * k), kIdescS, 1);
+                        }
+                    }
+                    if (elect_one()) tc_commit<1>(k_empty + 8 * (kc % kStages));
+                    __syncwarp();
                 }
-                tc_commit<1>(s_ready + 8 * (i & 1));
+                if (elect_one()) tc_commit<1>(s_ready + 8 * (i & 1));
+                __syncwarp();
             };
             auto pv = [&](int i) {
-                const unsigned a = tmem + kTmemS + 64 * (i & 1);
                 const unsigned later = (i * T::kKeys) % kFlushKeys != 0;   // 0: O starts afresh
-                for (int h = 0; h < T::kParts; h++) {
-                    const unsigned at = stage(53);
+#pragma unroll 1
+                for (int s = 0; s < 2 * T::kParts; s++, vc++) {   // half of the rows, part of the dims
+                    const int half = s / T::kParts, h = s % T::kParts;
+                    wait(v_full + 8 * (vc % kStages), (vc / kStages) & 1, 53);
+                    __syncwarp();
                     if (*wait.abort) return;
-                    const unsigned d = tmem + kTmemO + 128 * h;
-                    const unsigned hi = desc_lo_mn(at, T::kChunkBytes), lo = desc_lo_mn(at + T::kPlaneBytes, T::kChunkBytes);
+                    tc_fence_after();
+                    const unsigned a = tmem + kTmemS + 64 * (i & 1) + T::kVKeys * half, d = tmem + kTmemO + 128 * h;
+                    const unsigned at = smem_u32(smem + kOffV) + (vc % kStages) * kVStage;
+                    const unsigned hi = desc_lo_mn(at, T::kVChunkBytes), lo = desc_lo_mn(at + T::kVPlaneBytes, T::kVChunkBytes);
+                    if (elect_one()) {
 #pragma unroll
-                    for (int k = 0; k < T::kKeys / 16; k++) {   // 16 keys: two groups of eight rows
-                        tc_mma_ts<1>(d, a + 16 * k, desc_from(lo + 128 * k), kIdescO, k == 0 ? later : 1);
-                        tc_mma_ts<1>(d, a + 16 * k + 8, desc_from(hi + 128 * k), kIdescO, 1);
-                        tc_mma_ts<1>(d, a + 16 * k, desc_from(hi + 128 * k), kIdescO, 1);
+                        for (int k = 0; k < T::kVKeys / 16; k++) {   // 16 keys: two groups of eight rows
+                            tc_mma_ts<1>(d, a + 16 * k, desc_from(lo + 128 * k), kIdescO, (half | k) == 0 ? later : 1);
+                            tc_mma_ts<1>(d, a + 16 * k + 8, desc_from(hi + 128 * k), kIdescO, 1);
+                            tc_mma_ts<1>(d, a + 16 * k, desc_from(hi + 128 * k), kIdescO, 1);
+                        }
+                        tc_commit<1>(v_empty + 8 * (vc % kStages));
                     }
-                    release();
+                    __syncwarp();
                 }
-                tc_commit<1>(o_done + 8 * (i & 1));
+                if (elect_one()) tc_commit<1>(o_done + 8 * (i & 1));
+                __syncwarp();
             };
             qk(0);
             for (int i = 0; i < n && !*wait.abort; i++) {
                 if (i + 1 < n) qk(i + 1);
                 if (*wait.abort) break;
                 wait(w_ready + 8 * (i & 1), (i >> 1) & 1, 54);
+                __syncwarp();
                 if (*wait.abort) break;
                 tc_fence_after();
                 pv(i);
             }
+            __syncwarp();
             if (*wait.abort) {
-                tc_commit<1>(all_done);
+                if (elect_one()) tc_commit<1>(all_done);
                 for (unsigned spin = 0; spin < kSpinLimit && !mbar_try_wait(all_done, 0); spin++) {}
             }
         }
-    } else if (warp >= 8 && warp < 16) {
-        // ------------------------------------------------------------ planes
-        const int w8 = warp - 8;
-        unsigned c_raw = 0, c = 0;
-        float *const key_factor = reinterpret_cast<float *>(smem + kOffKey);
+    } else if (warp == 18) {
+        // ------------------------------------------------------------ the factors of V's rows, which the softmax wants early
         float *const value_power = reinterpret_cast<float *>(smem + kOffPow);
         float *const value_inverse = reinterpret_cast<float *>(smem + kOffInv);
-        auto take_stage = [&]() {
-            wait(st_empty + 8 * (c % kStages), ((c / kStages) & 1) ^ 1, 55);
-            return smem + kOffStages + (c % kStages) * kStageBytes;
-        };
-        auto give_stage = [&]() {
-            fence_async_shared();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(st_full + 8 * (c % kStages));
-            c++;
-        };
-        for (int m = 0; m < units; m++) {
-            const int t = unit_tile(m), live = tile_rows(t);
-            const bool is_v = unit_is_v(m);
-            if constexpr (kType == 0) {
-                // thread: block lane / 4 of row 4 * (warp - 8) + lane % 4
-                const int key = 4 * w8 + (lane & 3), blk = lane >> 2;
-                const unsigned mine = c_raw + (w8 >> 2), slot = mine % T::kRawSlots;
-                wait(raw_full + 8 * slot, (mine / T::kRawSlots) & 1, 56);
-                float x[32];   // an odd block's halves are swapped: eight lanes' words fall into different banks
-                const float4 *const src = reinterpret_cast<const float4 *>(smem + kOffRaw + slot * T::kRawSlot +
-                                                                           (key & 15) * T::kRowPitch + blk * 128);
-                float most = 0.0f;
-                bool bad = false;
-#pragma unroll
-                for (int j = 0; j < 8; j++) {
-                    float4 w = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                    if (key < live) w = src[j ^ ((blk & 1) << 2)];
-                    x[4 * j] = w.x;
-                    x[4 * j + 1] = w.y;
-                    x[4 * j + 2] = w.z;
-                    x[4 * j + 3] = w.w;
-#pragma unroll
-                    for (int e = 0; e < 4; e++) {
-                        most = fmaxf(most, fabsf(x[4 * j + e]));
-                        bad = bad || !(fabsf(x[4 * j + e]) < INFINITY);
-                    }
+        // Values' powers are taken relative to that of the run's first row: the exponents of the weights stay as small as
+        // the scores, to whose rounding they would add. (Within [-20, 16], which keeps the differences in range.)
+        int power0 = 0;
+#pragma unroll 1
+        for (int t = 0; t < n; t++) {
+            const int live = tile_rows(t);
+#pragma unroll 1
+            for (int j = 0; j < 2; j++) {
+                const unsigned u = raw_of(true, t) + j;
+                wait(raw_bar(true, 2 * t + j), ((2 * t + j) >> 3) & 1, 56);
+                const unsigned char *const from = smem + kOffRaw + (u % T::kRawSlots) * T::kRawSlot;
+                if (t == 0 && j == 0) {
+                    power0 = first_power<kType>(from, lane);
+                    if (lane == 0) s_power0 = power0;
                 }
+                // f32: a lane has half of a row; quantised: a lane has a row
+                const int r = kType == 0 ? lane & 15 : lane, key = T::kRawRows * j + r;
+                unsigned most = 0;
+                if (key < live) most = row_most<kType>(from + r * T::kRowPitch, kType == 0 ? lane >> 4 : 0);
+                if constexpr (kType == 0) most = max(most, __shfl_xor_sync(0xffffffffu, most, 16));
+                bool bad;
+                const int e = row_power<kType>(most, bad);
+                value_power[64 * (t % kFactors) + key] = bad ? 0.0f : (float)(e - power0);
+                value_inverse[64 * (t % kFactors) + key] = bad ? __int_as_float(0x7fffffff) : power(power0 - e);
                 __syncwarp();
-                if (lane == 0) mbar_arrive(raw_empty + 8 * slot);
-                c_raw += T::kPieces;
-#pragma unroll
-                for (int o = 4; o < 32; o <<= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
-                const unsigned whose = 0x11111111u << (lane & 3);
-                bad = (__ballot_sync(0xffffffffu, bad) & whose) != 0;
-                const int top = (__float_as_int(most) >> 23) & 255;
-                int e = min(max(top - 127 - 10, (int)kLeastPower), 116);   // (a row of zeros: the least)
-                if (bad) e = 0;
-                const float f = bad ? 0.0f : power(-e);
-                unsigned char *const st = take_stage();
-                if (blk == 0) {
-                    if (is_v) {
-                        value_power[64 * (t & 1) + key] = (float)e;
-                        value_inverse[64 * (t & 1) + key] = bad ? __int_as_float(0x7fffffff) : power(-e);
-                    } else {
-                        key_factor[64 * (t % 3) + key] = bad ? __int_as_float(0x7fffffff) : power(e);
-                    }
-                }
-                unsigned char *const dst = st + (blk >> 1) * T::kChunkBytes + key * 128;
-#pragma unroll
-                for (int j = 0; j < 4; j++) {
-                    unsigned h[4], l[4];
-#pragma unroll
-                    for (int k = 0; k < 4; k++)
-                        split_pair(bad ? 0.0f : x[8 * j + 2 * k] * f, bad ? 0.0f : x[8 * j + 2 * k + 1] * f, h[k], l[k]);
-                    const int u = 4 * (blk & 1) + (j ^ ((blk & 1) << 1));
-                    const int at = (u ^ (key & 7)) << 4;
-                    *reinterpret_cast<uint4 *>(dst + at) = make_uint4(h[0], h[1], h[2], h[3]);
-                    *reinterpret_cast<uint4 *>(dst + T::kPlaneBytes + at) = make_uint4(l[0], l[1], l[2], l[3]);
-                }
-                give_stage();
-            } else {
-                // thread: pair lane / 8 of row 8 * (warp - 8) + lane % 8; one block of it in each part
-                constexpr int kPair = kType == 1 ? 17 : 9, kOdd = kType == 1 ? 8 : 4;   // words; the odd block's first
-                const int key = 8 * w8 + (lane & 7), pair = lane >> 3;
-                const unsigned slot = c_raw % T::kRawSlots;
-                wait(raw_full + 8 * slot, (c_raw / T::kRawSlots) & 1, 56);
-                const unsigned *const src = reinterpret_cast<const unsigned *>(smem + kOffRaw + slot * T::kRawSlot +
-                                                                               key * T::kRowPitch) + pair * kPair;
-                unsigned w[kPair];
-#pragma unroll
-                for (int j = 0; j < kPair; j++) w[j] = key < live ? src[j] : 0u;
-                __syncwarp();
-                if (lane == 0) mbar_arrive(raw_empty + 8 * slot);
-                c_raw++;
-                const unsigned s0 = w[0] & 0xffffu, s1 = w[kOdd] >> 16;   // the scales' bits
-                int most = max((int)(s0 & 0x7fffu), (int)(s1 & 0x7fffu));
-                most = max(most, __shfl_xor_sync(0xffffffffu, most, 8));
-                most = max(most, __shfl_xor_sync(0xffffffffu, most, 16));
-                const bool bad = most >= 0x7c00;
-                // the row's largest scale comes to [8, 16): codes times it stay below 2^11 and lo is exact
-                int e = most == 0 ? (int)kLeastPower : max(most >> 10, 1) - 15 - 3;
-                if (bad) e = 0;
-                if (!is_v && most == 0) e = 0;
-                const float f = bad || most == 0 ? 0.0f : power(-e);
-#pragma unroll
-                for (int h = 0; h < 2; h++) {
-                    unsigned hi[16], lo[16];
-                    const float s = half_bits_to_float((uint16_t)(h ? s1 : s0));
-                    block_planes<kType>(w + (h ? kOdd : 0), h != 0, __float2half2_rn(bad ? 0.0f : s * f), hi, lo);
-                    unsigned char *const st = take_stage();
-                    if (h == 0 && pair == 0) {
-                        if (is_v) {
-                            value_power[64 * (t & 1) + key] = (float)e;
-                            value_inverse[64 * (t & 1) + key] = bad ? __int_as_float(0x7fffffff) : power(-e);
-                        } else {
-                            key_factor[64 * (t % 3) + key] = bad ? __int_as_float(0x7fffffff) : power(e);
-                        }
-                    }
-                    unsigned char *const dst = st + (pair >> 1) * T::kChunkBytes + key * 128;
-#pragma unroll
-                    for (int j = 0; j < 4; j++) {
-                        const int at = ((4 * (pair & 1) + j) ^ (key & 7)) << 4;
-                        *reinterpret_cast<uint4 *>(dst + at) = make_uint4(hi[4 * j], hi[4 * j + 1], hi[4 * j + 2], hi[4 * j + 3]);
-                        *reinterpret_cast<uint4 *>(dst + T::kPlaneBytes + at) =
-                            make_uint4(lo[4 * j], lo[4 * j + 1], lo[4 * j + 2], lo[4 * j + 3]);
-                    }
-                    give_stage();
-                }
+                if (lane == 0) mbar_arrive(raw_empty + 8 * (u % T::kRawSlots));
             }
-            if (is_v) {   // this tile's factors of K and V are there
-                if (lane == 0) mbar_arrive(factors + 8 * (t & 1));
+            if (lane == 0) mbar_arrive(factors + 8 * (t % kFactors));
+        }
+    } else if (warp >= 8 && warp < 16) {
+        // ------------------------------------------------------------ planes: warps 8-11 of K, 12-15 of V
+        const bool is_v = warp >= 12;
+        const int w4 = warp & 3;
+        float *const key_factor = reinterpret_cast<float *>(smem + kOffKey);
+        // half tile i of this kind, in raw slot u: waits until it is there
+        auto raw = [&](int i, unsigned u) {
+            wait(raw_bar(is_v, i), (i >> 3) & 1, 56);
+            return smem + kOffRaw + (u % T::kRawSlots) * T::kRawSlot;
+        };
+        auto free_raw = [&](unsigned u, int times) {
+            __syncwarp();
+            if (lane == 0)
+                for (int i = 0; i < times; i++) mbar_arrive(raw_empty + 8 * (u % T::kRawSlots));
+        };
+        constexpr int kPair = kType == 1 ? 17 : 9, kOdd = kType == 1 ? 8 : 4;   // words of two blocks; the odd block's first
+        // Thread's row of half tile j. f32: block lane / 4 of row 4 (warp % 4) + lane % 4 (of 16). Quantised: pair lane / 8 of
+        // row 8 (warp % 4) + lane % 8 (of 32), one block of it in each part.
+        const int row = kType == 0 ? 4 * w4 + (lane & 3) : 8 * w4 + (lane & 7);
+        const int blk = lane >> 2, pair = lane >> 3;
+        const bool first = (kType == 0 ? blk : pair) == 0;   // the lane that speaks for a row
+        // the largest of the thread's part of a row
+        auto most_of = [&](const unsigned char *from, bool live) {
+            unsigned m = 0;
+            if (!live) return m;
+            if constexpr (kType == 0) {
+                const uint4 *const src = reinterpret_cast<const uint4 *>(from + blk * 128);
+#pragma unroll
+                for (int k = 0; k < 8; k++) {
+                    const uint4 x = src[k ^ ((blk & 1) << 2)];   // (eight lanes' words fall into different banks)
+                    m = max(max(m, x.x & 0x7fffffffu), max(max(x.y & 0x7fffffffu, x.z & 0x7fffffffu), x.w & 0x7fffffffu));
+                }
+            } else {
+                const unsigned *const src = reinterpret_cast<const unsigned *>(from) + pair * kPair;
+                m = max(src[0] & 0x7fffu, (src[kOdd] >> 16) & 0x7fffu);
+            }
+            return m;
+        };
+        if (!is_v && n > 0) named_sync(7, 12 * 32);   // Q hi has left K's stages
+        unsigned c = 0;                               // stages written
+#pragma unroll 1
+        for (int t = 0; t < n; t++) {
+            const int live = tile_rows(t);
+            const unsigned u0 = raw_of(is_v, t);   // the tile's first raw slot
+            const unsigned char *from[2];
+            float f[2], factor[2];
+#pragma unroll
+            for (int j = 0; j < 2; j++) {
+                const int key = T::kRawRows * j + row;
+                from[j] = raw(2 * t + j, u0 + j) + row * T::kRowPitch;
+                unsigned most = most_of(from[j], key < live);
+#pragma unroll
+                for (int o = kType == 0 ? 4 : 8; o < 32; o <<= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
+                bool bad;
+                const int e = row_power<kType>(most, bad);
+                f[j] = bad || (kType != 0 && e == kLeastPower) || key >= live ? 0.0f : power(-e);
+                factor[j] = bad ? __int_as_float(0x7fffffff) : power(e);
+            }
+            // K: both halves of a part, then the other part; V: both parts of a half, then the other half
+#pragma unroll 1
+            for (int s = 0; s < 2 * T::kParts; s++) {
+                const int j = kType == 0 ? s : (is_v ? s >> 1 : s & 1), h = kType == 0 ? 0 : (is_v ? s & 1 : s >> 1);
+                const int key = T::kRawRows * j + row;
+                const unsigned full = (is_v ? v_full : k_full) + 8 * (c % kStages);
+                if (is_v || j == 0) {
+                    wait((is_v ? v_empty : k_empty) + 8 * (c % kStages), ((c / kStages) & 1) ^ 1, 55);
+                    if (!is_v && s == 0 && first) {
+#pragma unroll
+                        for (int i = 0; i < 2; i++) key_factor[64 * (t % kFactors) + T::kRawRows * i + row] = factor[i];
+                    }
+                }
+                const int chunk = kType == 0 ? blk >> 1 : pair >> 1;
+                unsigned char *const dst = is_v ? smem + kOffV + (c % kStages) * kVStage + row * 128 + chunk * T::kVChunkBytes
+                                                : smem + kOffK + (c % kStages) * kKStage + key * 128 + chunk * T::kChunkBytes;
+                const int plane = is_v ? T::kVPlaneBytes : T::kPlaneBytes;
+                const float by = j ? f[1] : f[0];
+                const unsigned char *const raw_row = j ? from[1] : from[0];
+                if constexpr (kType == 0) {
+                    // (an odd block's halves are swapped, as above)
+                    const float4 *const src = reinterpret_cast<const float4 *>(raw_row + blk * 128);
+#pragma unroll
+                    for (int k = 0; k < 4; k++) {
+                        const float4 a = src[(2 * k) ^ ((blk & 1) << 2)], b = src[(2 * k + 1) ^ ((blk & 1) << 2)];
+                        const float v[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+                        unsigned hi[4], lo[4];
+#pragma unroll
+                        for (int d = 0; d < 4; d++) {
+                            split_pair(v[2 * d] * by, v[2 * d + 1] * by, hi[d], lo[d]);
+                            if (by == 0.0f) hi[d] = lo[d] = 0;   // (not finite, or no row at all)
+                        }
+                        const int unit = 4 * (blk & 1) + (k ^ ((blk & 1) << 1));
+                        const int at = (unit ^ (key & 7)) << 4;
+                        *reinterpret_cast<uint4 *>(dst + at) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+                        *reinterpret_cast<uint4 *>(dst + plane + at) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+                    }
+                } else {
+                    const unsigned *const src = reinterpret_cast<const unsigned *>(raw_row) + pair * kPair + (h ? kOdd : 0);
+                    unsigned w[kOdd + 1], hi[16], lo[16];
+#pragma unroll
+                    for (int k = 0; k <= kOdd; k++) w[k] = src[k];
+                    const float scale = half_bits_to_float((uint16_t)(w[0] >> (16 * h)));
+                    block_planes<kType>(w, h ? 0x7654 : 0x5432, __float2half2_rn(by == 0.0f ? 0.0f : scale * by), hi, lo);
+#pragma unroll
+                    for (int k = 0; k < 4; k++) {
+                        const int at = ((4 * (pair & 1) + k) ^ (key & 7)) << 4;
+                        *reinterpret_cast<uint4 *>(dst + at) = make_uint4(hi[4 * k], hi[4 * k + 1], hi[4 * k + 2], hi[4 * k + 3]);
+                        *reinterpret_cast<uint4 *>(dst + plane + at) =
+                            make_uint4(lo[4 * k], lo[4 * k + 1], lo[4 * k + 2], lo[4 * k + 3]);
+                    }
+                }
+                const bool done = s + 1 == 2 * T::kParts;
+                if (is_v || j == 1) {   // the stage is written
+                    fence_async_shared();
+                    __syncwarp();
+                    if (lane == 0) {
+                        mbar_arrive(full);
+                        if (!is_v && done) mbar_arrive(factors + 8 * (t % kFactors));
+                    }
+                    c++;
+                }
+                // a half's rows were read for the last time
+                if (done || (is_v && T::kParts == 2 && s == 1) || (kType == 0)) free_raw(u0 + j, warp == 8 ? 2 : 1);
+                if (!is_v && T::kParts == 2 && done) free_raw(u0, warp == 8 ? 2 : 1);
             }
         }
     } else if (warp < 8 && n > 0) {
@@ -567,10 +702,17 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tree_tc(TreeParams p) {
         };
         // dims of column group j (32 columns) of this thread's half of O
         auto dims_of = [&](int j) { return kType == 0 ? 128 * half + 32 * j : 32 * T::block(half, j); };
+        const bool idle = 32 * (warp & 3) >= rows;   // (no row of this warp is live: nothing reads its lanes)
+#pragma unroll 1
         for (int i = 0; i < n; i++) {
             const unsigned s_at = lane_at + kTmemS + 64 * (i & 1) + T::kHalf * half;
             wait(s_ready + 8 * (i & 1), (i >> 1) & 1, 57);
-            wait(factors + 8 * (i & 1), (i >> 1) & 1, 58);
+            if (idle) {
+                __syncwarp();
+                if (lane == 0) mbar_arrive(w_ready + 8 * (i & 1));
+                continue;
+            }
+            wait(factors + 8 * (i % kFactors), (i / kFactors) & 1, 58);
             __syncwarp();
             tc_fence_after();
             float u[T::kHalf];
@@ -582,9 +724,9 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tree_tc(TreeParams p) {
             } else {
                 tmem_ld16(s_at, u);
             }
-            const float4 *const kf = reinterpret_cast<const float4 *>(smem + kOffKey) + 16 * (i % 3) + T::kHalf / 4 * half;
-            const float4 *const vp = reinterpret_cast<const float4 *>(smem + kOffPow) + 16 * (i & 1) + T::kHalf / 4 * half;
-            const float4 *const vi = reinterpret_cast<const float4 *>(smem + kOffInv) + 16 * (i & 1) + T::kHalf / 4 * half;
+            const float4 *const kf = reinterpret_cast<const float4 *>(smem + kOffKey) + 16 * (i % kFactors) + T::kHalf / 4 * half;
+            const float4 *const vp = reinterpret_cast<const float4 *>(smem + kOffPow) + 16 * (i % kFactors) + T::kHalf / 4 * half;
+            const float4 *const vi = reinterpret_cast<const float4 *>(smem + kOffInv) + 16 * (i % kFactors) + T::kHalf / 4 * half;
 #pragma unroll
             for (int e = 0; e < T::kHalf; e += 4) {
                 const float4 f = kf[e / 4], g = vp[e / 4];
@@ -699,52 +841,56 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tree_tc(TreeParams p) {
             if (lane == 0) mbar_arrive(w_ready + 8 * (i & 1));
         }
         // ------------------------------------------------------------ epilogue
-        l += meet(n, l);
         wait(o_done + 8 * ((n - 1) & 1), ((n - 1) >> 1) & 1, 59);
         __syncwarp();
-        tc_fence_after();
-        // O leaves through shared memory: whole rows of 1 KB by bulk copies (the planes and Q are dead: every MMA is done)
+        // O leaves through shared memory, where a thread has half a row, in whole rows of 1 KB (the planes and Q are dead:
+        // every MMA is done)
         float *const staged = reinterpret_cast<float *>(smem);
-        const bool apart = m_out != -INFINITY;   // part of the row is in memory
-        const float g = apart ? exp2f(m - m_out) : 1.0f;
-        const float inv = whole ? 1.0f / l : 1.0f;
-        // (where the last part outweighs what is in memory past all bounds, that is dropped)
-        const bool drop = apart && m > m_out + 60.0f;
+        if (!idle) {
+            tc_fence_after();
+            l += meet(n, l);
+            // (O lacks the power that the values' are relative to)
+            const float inv = whole ? power(s_power0) / l : power(s_power0);
+            // part of the row may be in memory; where the last part outweighs that past all bounds, it is dropped
+            const bool join = m_out != -INFINITY && m <= m_out + 60.0f;
+            const float g = join ? exp2f(m_out - m) : 0.0f;
 #pragma unroll 1
-        for (int j = 0; j < 4; j++) {
-            unsigned v[32];
-            tmem_ld32(lane_at + kTmemO + 128 * half + 32 * j, v);
-            float *const at = staged + r * kOutPitch + dims_of(j);
-            if (live && !*wait.abort) {
-#pragma unroll
-                for (int e = 0; e < 32; e += 4) {
-                    float4 w = make_float4(__uint_as_float(v[e]), __uint_as_float(v[e + 1]), __uint_as_float(v[e + 2]),
-                                           __uint_as_float(v[e + 3]));
-                    if (apart && !drop) {
-                        // (this thread's own stores and additions)
+            for (int j = 0; j < 4; j++) {
+                unsigned v[32];
+                tmem_ld32(lane_at + kTmemO + 128 * half + 32 * j, v);
+                float *const at = staged + r * kOutPitch + dims_of(j);
+                if (join && live) {
+                    // (this thread's own stores and additions)
+#pragma unroll 1
+                    for (int e = 0; e < 32; e += 4) {
                         const float4 old = __ldcg(reinterpret_cast<const float4 *>(dst + dims_of(j) + e));
-                        w.x = fmaf(w.x, g, old.x);
-                        w.y = fmaf(w.y, g, old.y);
-                        w.z = fmaf(w.z, g, old.z);
-                        w.w = fmaf(w.w, g, old.w);
+                        *reinterpret_cast<float4 *>(at + e) = make_float4(old.x * g, old.y * g, old.z * g, old.w * g);
                     }
-                    const float s = apart && !drop ? inv / g : inv;
-                    *reinterpret_cast<float4 *>(at + e) = make_float4(w.x * s, w.y * s, w.z * s, w.w * s);
+#pragma unroll
+                    for (int e = 0; e < 32; e++) v[e] = __float_as_uint(__uint_as_float(v[e]) + at[e]);
                 }
+#pragma unroll
+                for (int e = 0; e < 32; e += 4)
+                    *reinterpret_cast<float4 *>(at + e) =
+                        make_float4(__uint_as_float(v[e]) * inv, __uint_as_float(v[e + 1]) * inv,
+                                    __uint_as_float(v[e + 2]) * inv, __uint_as_float(v[e + 3]) * inv);
+            }
+            if (live && half == 0 && !whole && !*wait.abort) {
+                const size_t at = 2 * ((size_t)blockIdx.x * kRows + r);
+                p.part_ml[at] = m;
+                p.part_ml[at + 1] = l;
             }
         }
-        if (live && half == 0 && !whole && !*wait.abort) {
-            const size_t at = 2 * ((size_t)blockIdx.x * kRows + r);
-            p.part_ml[at] = m;
-            p.part_ml[at + 1] = l;
-        }
-        fence_async_shared();
         named_sync(1, 256);
-        if (!*wait.abort && lane == 0) {
-            for (int rr = warp; rr < rows; rr += 8)
-                bulk_store(whole ? p.out + head_row(rr) * kD : p.part_acc + ((size_t)blockIdx.x * kRows + rr) * kD,
-                           smem_u32(staged + rr * kOutPitch), kD * 4);
-            bulk_store_commit_wait_read();
+        if (!*wait.abort) {
+#pragma unroll 2
+            for (int rr = warp; rr < rows; rr += 8) {
+                float4 *const to = reinterpret_cast<float4 *>(whole ? p.out + head_row(rr) * kD
+                                                                    : p.part_acc + ((size_t)blockIdx.x * kRows + rr) * kD);
+                const float4 *const from = reinterpret_cast<const float4 *>(staged + rr * kOutPitch);
+                to[lane] = from[lane];
+                to[lane + 32] = from[lane + 32];
+            }
         }
     }
     tc_fence_before();

@@ -930,7 +930,7 @@ size_t hipml_attn_tree_workspace_bytes(int n_heads, int n_kv, int head_dim, int 
     const int grid_tc = head_dim == 256 ? tree_grid_of(true, n_heads, n_kv, nodes, slots) : 0;
     if (grid < 0 || grid_tc < 0) return 0;
     const size_t rows = (size_t)grid * kTreeScalarRows, rows_tc = (size_t)grid_tc * kTreeTcRows;
-    return (rows > rows_tc ? rows : rows_tc) * (head_dim + 2) * sizeof(float);
+    return (size_t)slots * sizeof(int4) + (rows > rows_tc ? rows : rows_tc) * (head_dim + 2) * sizeof(float);
 }
 
 int hipml_attn_tree(hipml_stream_t stream, int kv_dtype, const int *pos, const int *parents, const float *q,
@@ -975,7 +975,8 @@ int hipml_attn_tree(hipml_stream_t stream, int kv_dtype, const int *pos, const i
     const bool tensor_core = head_dim == 256 && (align & 15) == 0;
     p.tile_rows = tensor_core ? kTreeTcRows : kTreeScalarRows;
     p.grid = tree_grid_of(tensor_core, n_heads, n_kv, nodes, slots);
-    p.part_acc = (float *)workspace;
+    p.shares = (int4 *)workspace;
+    p.part_acc = (float *)(p.shares + slots);
     p.part_ml = p.part_acc + (size_t)p.grid * p.tile_rows * head_dim;
     if (int e = (tensor_core ? launch_tree_tc : launch_tree_scalar)(as_stream(stream), p)) return e;
     return launch_tree_fold(as_stream(stream), p);

@@ -24,6 +24,7 @@ struct TreeParams {
     float *out;            // as q
     float *part_acc;       // [grid][tile_rows][head_dim]
     float *part_ml;        // [grid][tile_rows] {maximum in log2 units, sum}
+    int4 *shares;          // [slots] {first CTA, runs, tiles}: how a slot was dealt out, for the fold
     int *status;
     int n_heads, n_kv, group, head_dim, stride, nodes, slots;
     int kv_dtype;          // 0 f32 [row][n_kv * head_dim], 1 q8_0, 2 q4_0 (head-major)
@@ -59,28 +60,41 @@ __device__ __forceinline__ TreeSlot tree_slot(const int *pos, int slot, int stri
 
 // One CTA's share: the query rows [tile * tile_rows, ...) of KV head kvh of a slot, over key tiles of run `run` of `runs`.
 struct TreeItem {
-    int slot, kvh, tile, run, runs, first;   // first: the CTA of run 0
+    int slot, kvh, tile, run, runs;
     int base, live, quota;
 };
 
+// The slots as a warp's lanes hold them: the first 32 stay in registers, so that the plan is one trip to memory.
+struct TreeSlots {
+    const TreeParams &p;
+    TreeSlot mine;
+    __device__ __forceinline__ explicit TreeSlots(const TreeParams &params) : p(params), mine({0, 0}) {
+        const int lane = threadIdx.x & 31;
+        if (lane < p.slots) mine = tree_slot(p.pos, lane, p.stride, p.nodes);
+    }
+    __device__ __forceinline__ TreeSlot at(int s) const {   // s % 32 == lane
+        return s < 32 ? mine : tree_slot(p.pos, s, p.stride, p.nodes);
+    }
+};
+
 // Key tiles per run, the same for all: the fewest with which the runs fit the grid. Called by a whole warp.
-__device__ __forceinline__ int tree_quota(const TreeParams &p) {
+__device__ __forceinline__ int tree_quota(const TreeParams &p, const TreeSlots &slots) {
     const int lane = threadIdx.x & 31;
     auto each = [&](auto f) {   // sum over the slots of f(key tiles, row tiles)
         int n = 0;
         for (int s = lane; s < p.slots; s += 32) {
-            const TreeSlot t = tree_slot(p.pos, s, p.stride, p.nodes);
+            const TreeSlot t = slots.at(s);
             n += f(div_up_int(t.base + t.live, kTreeKeyTile), div_up_int(t.live * p.group, p.tile_rows));
         }
         return (int)__reduce_add_sync(0xffffffffu, n);
     };
     const int fit = p.grid / p.n_kv;   // runs per KV head
     const int total = each([](int keys, int rows) { return keys * rows; });
-    const int few = each([](int, int rows) { return rows; });
     auto runs_at = [&](int q) { return each([&](int keys, int rows) { return rows * div_up_int(keys, q); }); };
     int lo = max(1, div_up_int(total, fit));
     if (runs_at(lo) <= fit) return lo;
     // sum(rows * ceil(keys / q)) <= total / q + few; with one run each, every triple has its CTA
+    const int few = each([](int, int rows) { return rows; });
     int hi = fit > few ? div_up_int(total, fit - few) : div_up_int(p.stride, kTreeKeyTile);
     hi = max(hi, lo + 1);
     while (hi - lo > 1) {
@@ -94,16 +108,18 @@ __device__ __forceinline__ int tree_ctas(const TreeParams &p, const TreeSlot &t,
     return p.n_kv * div_up_int(t.live * p.group, p.tile_rows) * div_up_int(t.base + t.live, kTreeKeyTile * quota);
 }
 
-// CTA `cta`'s item (slot < 0: none). Called by a whole warp.
-__device__ __forceinline__ TreeItem tree_item(const TreeParams &p, int quota, int cta) {
+// CTA `cta`'s item (slot < 0: none); a slot's first CTA leaves its share for the fold. Called by a whole warp.
+__device__ __forceinline__ TreeItem tree_item(const TreeParams &p, int cta) {
     const int lane = threadIdx.x & 31;
+    const TreeSlots slots(p);
+    const int quota = tree_quota(p, slots);
     TreeItem it;
     it.slot = -1;
     it.quota = quota;
     int before = 0;
     for (int s0 = 0; s0 < p.slots && it.slot < 0; s0 += 32) {
         TreeSlot t = {0, 0};
-        if (s0 + lane < p.slots) t = tree_slot(p.pos, s0 + lane, p.stride, p.nodes);
+        if (s0 + lane < p.slots) t = slots.at(s0 + lane);
         const int mine = tree_ctas(p, t, quota);
         int upto = mine;
 #pragma unroll
@@ -124,23 +140,19 @@ __device__ __forceinline__ TreeItem tree_item(const TreeParams &p, int quota, in
             it.run = in_slot - triple * it.runs;
             it.kvh = triple / tiles;
             it.tile = triple - it.kvh * tiles;
-            it.first = cta - it.run;
+            if (in_slot == 0 && lane == 0) p.shares[it.slot] = make_int4(cta, it.runs, tiles, 0);
         }
         before += __shfl_sync(0xffffffffu, upto, 31);
     }
     return it;
 }
 
-// Bits of the drafted rows that `node` sees: its own and those of its ancestors, into `words`. A parent that is no earlier
-// node ends the walk (and is reported).
-__device__ __forceinline__ void tree_ancestors(const int *parents, int node, unsigned (&words)[kTreeWords], int *status) {
-#pragma unroll
+// Bits of the drafted rows that `node` sees, its own and those of its ancestors, into words[kTreeWords]. A parent that is no
+// earlier node ends the walk (and is reported).
+__device__ __forceinline__ void tree_ancestors(const int *parents, int node, unsigned *words, int *status) {
     for (int w = 0; w < kTreeWords; w++) words[w] = 0;
-    int i = node;
-    while (i >= 0) {
-#pragma unroll
-        for (int w = 0; w < kTreeWords; w++)
-            if ((i >> 5) == w) words[w] |= 1u << (i & 31);
+    for (int i = node; i >= 0;) {
+        words[i >> 5] |= 1u << (i & 31);
         const int up = parents[i];
         if (up >= i || up < -1) {
             atomicCAS(status, 0, kTreeBadTree);
