@@ -62,7 +62,7 @@ __global__ void __launch_bounds__(256) attn_tree_scalar(TreeParams p) {
     griddep_wait();
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     if (warp == 0) {
-        const TreeItem it = tree_item(p, blockIdx.x);
+        const TreeItem it = tree_item<kRows>(p, blockIdx.x);
         if (lane == 0) s_item = it;
     }
     __syncthreads();
@@ -75,7 +75,7 @@ __global__ void __launch_bounds__(256) attn_tree_scalar(TreeParams p) {
     const size_t slot_row = (size_t)it.slot * p.nodes;
     // a row of the tile as a row of q and out, in heads
     auto head_row = [&](int r) {
-        const int at = it.tile * kRows + r, node = at / p.group;
+        const int at = it.tile * kRows + r, node = p.node_of(at);
         return (slot_row + node) * p.n_heads + it.kvh * p.group + (at - node * p.group);
     };
     for (int i = tid; i < kRows * kD; i += 256) {
@@ -84,7 +84,7 @@ __global__ void __launch_bounds__(256) attn_tree_scalar(TreeParams p) {
     }
     __syncthreads();
     if (tid < rows) {
-        tree_ancestors(s_parents, (it.tile * kRows + tid) / p.group, s_sees[tid], p.status);
+        tree_ancestors(s_parents, p.node_of(it.tile * kRows + tid), s_sees[tid], p.status);
     }
     const unsigned char *const kc = p.k + (size_t)it.slot * p.slot_bytes, *const vc = p.v + (size_t)it.slot * p.slot_bytes;
     float acc[kWarpRows][kB], m[kWarpRows], l[kWarpRows];

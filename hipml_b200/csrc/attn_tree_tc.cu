@@ -16,8 +16,8 @@
 // f16 parts need their operands in range whatever the cache holds. So each key and each value row is scaled by a power of two
 // of its own, by its largest scale (f32: value), and each query row too. S is multiplied back (a factor per key and one
 // per row); the value's power 2^E goes into the weight: w = 2^(s + E - m), where m follows the largest s + E, and the
-// denominator takes w 2^-E. A row that is not finite is zero in the planes and its factors are not a number, so it reaches
-// the rows that see it and no others (a hidden key's weight is 0, and 0 times its plane is 0).
+// denominator takes w 2^-E. A row that is not finite is zero in the planes and its factor (or power) is not a number, so it
+// reaches the rows that see it and no others (a hidden key's weight is 0, and 0 times its plane is 0).
 //
 // Where the time goes (a quantised tile of 64 rows): tensor pipe 2 x 1,536 cycles; shared memory 7.1 KB a row: the raw
 // bytes in and out (1.1), the planes (2), K and the low part of Q into the pipe (2.5), V (1.5), 55 cycles a row at 128
@@ -27,9 +27,10 @@
 // Sums: the tensor cores cut their f32 accumulators off instead of rounding them, 3.5e-9 relative per key of an unbroken
 // chain, so every kFlushKeys keys O leaves TMEM for the run's partial in memory (added there, in f32).
 //
-// Warps 0-7 softmax and epilogue, 8-11 planes of K, 12-15 of V, 16 copies, 17 MMAs (the whole warp runs that loop and one
-// elected lane issues: from a branch of a single lane every descriptor went through a move to the uniform registers, 46
-// cycles an MMA of N = 64 and 83 beside the other warps, against 32), 18 the factors of V's rows. Waits are bounded: one that runs out sets the device
+// Warps 0-7 softmax and epilogue, 8-11 planes of K, 12-15 of V, 16 copies, 17 the factors of V's rows, 19 MMAs
+// (the whole warp runs that loop and one elected lane issues: from a branch of a single lane every descriptor went through a
+// move to the uniform registers, 46 cycles an MMA of N = 64 and 83 beside the other warps, against 32; the fourth scheduler
+// has the fewest other warps). Waits are bounded: one that runs out sets the device
 // status and a flag that turns every other wait of the CTA into none; all warps still come to every barrier, nothing is
 // written out, and copies and MMAs in flight are waited for (bounded too) before shared memory and TMEM are released.
 #include <atomic>
@@ -45,7 +46,7 @@ namespace {
 using namespace ptx;
 
 constexpr int kD = 256, kRows = kTreeTcRows;
-constexpr int kThreads = 19 * 32;
+constexpr int kThreads = 20 * 32;
 constexpr int kGroup = 4;                        // warps that make planes: four of K, four of V
 constexpr int kQChunk = kRows * 128;             // 128 rows x 64 dims, f16
 constexpr int kQBytes = 4 * kQChunk;             // one plane of Q
@@ -115,14 +116,15 @@ __device__ __forceinline__ unsigned desc_lo_mn(unsigned addr, unsigned pitch) {
 
 // The kernel's code is kept small: its roles together, and what runs once, come through one instruction cache (with every
 // loop unrolled a tile of 64 rows took 10,000 cycles and Q 6,700). Loops over blocks, rows and chunks are loops.
-__device__ __noinline__ void wait_long(unsigned bar, unsigned parity, volatile int *abort, int *status, int code) {
+__device__ __noinline__ bool wait_long(unsigned bar, unsigned parity, volatile int *abort, int *status, int code) {
     for (unsigned i = 0; i < kSpinLimit; i++) {
-        if (mbar_try_wait(bar, parity)) return;
-        if ((i & 255) == 255 && *abort) return;
+        if (mbar_try_wait(bar, parity)) return true;
+        if ((i & 255) == 255 && *abort) return false;
         if (i > 4096) __nanosleep(64);
     }
     atomicCAS(status, 0, code);
     *abort = 1;
+    return false;
 }
 __device__ __forceinline__ bool elect_one() {
     unsigned p;
@@ -136,8 +138,8 @@ __device__ __forceinline__ bool elect_one() {
 struct Waits {
     volatile int *abort;
     int *status;
-    __device__ __forceinline__ void operator()(unsigned bar, unsigned parity, int code) const {
-        if (!mbar_try_wait(bar, parity)) wait_long(bar, parity, abort, status, code);
+    __device__ __forceinline__ bool operator()(unsigned bar, unsigned parity, int code) const {
+        return mbar_try_wait(bar, parity) || wait_long(bar, parity, abort, status, code);
     }
 };
 
@@ -258,31 +260,23 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tree_tc(TreeParams p) {
                    factors = smem_u32(bars + 38), all_done = smem_u32(bars + 42);
     static_assert(T::kRawSlots <= 8 && kFactors <= 4 && kBars == 43, "barriers");
     auto raw_bar = [&](bool v, int i) { return raw_full + 8 * ((v ? 8 : 0) + (i & 7)); };   // of half tile i
-    if (tid == 0) {
-        for (int i = 0; i < 16; i++) mbar_init(raw_full + 8 * i, 1);
-        for (int i = 0; i < T::kRawSlots; i++) {
-            // four warps make planes of a slot's rows; warp 18 reads V's as well (and K's first warp arrives once more)
-            mbar_init(raw_empty + 8 * i, kGroup + 1);
+    if (warp == 1) {
+        // four warps make planes of a raw slot's rows; warp 17 reads V's as well (and K's first warp arrives once more)
+        for (int i = lane; i < kBars; i += 32) {
+            const int kind = i / 2;   // from 12 on: pairs of k_full, k_empty, v_full, v_empty, s_ready, w_ready, o_done
+            mbar_init(raw_full + 8 * i, i < 16 ? 1 : i < 24 || (i >= 38 && i < 42) ? kGroup + 1
+                                                   : kind == 12 || kind == 14    ? kGroup
+                                                   : kind == 17                  ? 8
+                                                                                 : 1);
         }
-        for (int i = 0; i < 2; i++) {
-            mbar_init(k_full + 8 * i, kGroup);
-            mbar_init(k_empty + 8 * i, 1);
-            mbar_init(v_full + 8 * i, kGroup);
-            mbar_init(v_empty + 8 * i, 1);
-            mbar_init(s_ready + 8 * i, 1);
-            mbar_init(w_ready + 8 * i, 8);
-            mbar_init(o_done + 8 * i, 1);
-        }
-        for (int i = 0; i < kFactors; i++) mbar_init(factors + 8 * i, kGroup + 1);
-        mbar_init(all_done, 1);
-        s_abort = 0;
+        if (lane == 0) s_abort = 0;
         mbar_init_fence();
     }
-    if (warp == 17) tmem_alloc<1>(smem_u32(&s_tmem), 512);
+    if (warp == 19) tmem_alloc<1>(smem_u32(&s_tmem), 512);
     tc_fence_before();
     griddep_wait();
     if (warp == 0) {
-        const TreeItem it = tree_item(p, blockIdx.x);
+        const TreeItem it = tree_item<kRows>(p, blockIdx.x);
         if (lane == 0) s_item = it;
     }
     __syncthreads();
@@ -295,7 +289,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tree_tc(TreeParams p) {
     const int n = it.slot < 0 ? 0 : (hi_key - lo_key + T::kKeys - 1) / T::kKeys;   // tiles
     const size_t first_node = (size_t)it.slot * p.nodes;
     auto head_row = [&](int r) {   // row r of the tile as a row of q and out, in heads
-        const int at = it.tile * kRows + r, node = at / p.group;
+        const int at = it.tile * kRows + r, node = p.node_of(at);
         return (first_node + node) * p.n_heads + it.kvh * p.group + (at - node * p.group);
     };
     // Half tiles in the raw ring: K0 K1 V0 K2 V1 .. V(n-1). A slot of V is free when its planes are made, in the middle of
@@ -359,7 +353,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tree_tc(TreeParams p) {
             reinterpret_cast<int *>(smem + kOffParents)[i] = p.parents[first_node + i];
         if (tid >= rows && tid < kRows) reinterpret_cast<float *>(smem + kOffRowFac)[tid] = 0.0f;
         auto row_at = [&](int r) { return reinterpret_cast<const float4 *>(p.q + head_row(r) * kD) + 2 * lane; };
-        constexpr int kAhead = 3;   // rows on their way
+        constexpr int kAhead = 4;   // rows on their way
         float4 x[kAhead][2];
 #pragma unroll
         for (int k = 0; k < kAhead; k++) {
@@ -368,37 +362,37 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tree_tc(TreeParams p) {
             x[k][1] = __ldg(src + 1);
         }
 #pragma unroll 1
-        for (int r = qw; r < rows; r += kQWarps) {
-            const float v[8] = {x[0][0].x, x[0][0].y, x[0][0].z, x[0][0].w, x[0][1].x, x[0][1].y, x[0][1].z, x[0][1].w};
+        for (int r0 = qw; r0 < rows; r0 += kQWarps * kAhead) {
 #pragma unroll
-            for (int k = 0; k + 1 < kAhead; k++) {
-                x[k][0] = x[k + 1][0];
-                x[k][1] = x[k + 1][1];
-            }
-            if (r + kQWarps * kAhead < rows) {
-                const float4 *const src = row_at(r + kQWarps * kAhead);
-                x[kAhead - 1][0] = __ldg(src);
-                x[kAhead - 1][1] = __ldg(src + 1);
-            }
-            unsigned most = 0;
+            for (int k = 0; k < kAhead; k++) {
+                const int r = r0 + kQWarps * k;
+                if (r >= rows) break;
+                const float v[8] = {x[k][0].x, x[k][0].y, x[k][0].z, x[k][0].w, x[k][1].x, x[k][1].y, x[k][1].z, x[k][1].w};
+                if (r + kQWarps * kAhead < rows) {
+                    const float4 *const src = row_at(r + kQWarps * kAhead);
+                    x[k][0] = __ldg(src);
+                    x[k][1] = __ldg(src + 1);
+                }
+                unsigned most = 0;
 #pragma unroll
-            for (int e = 0; e < 8; e++) most = max(most, __float_as_uint(v[e]) & 0x7fffffffu);
-            most = __reduce_max_sync(0xffffffffu, most);
-            const bool bad = most >= 0x7f800000u;
-            // the row's largest value comes to [2^10, 2^11)
-            const int e = min(max((int)(most >> 23) - 127 - 10, -116), 116);
-            const float f = power(-e);
-            unsigned hi[4], lo[4];
+                for (int e = 0; e < 8; e++) most = max(most, __float_as_uint(v[e]) & 0x7fffffffu);
+                most = __reduce_max_sync(0xffffffffu, most);
+                const bool bad = most >= 0x7f800000u;
+                // the row's largest value comes to [2^10, 2^11)
+                const int e = min(max((int)(most >> 23) - 127 - 10, -116), 116);
+                const float f = power(-e);
+                unsigned hi[4], lo[4];
 #pragma unroll
-            for (int d = 0; d < 4; d++) {
-                split_pair(v[2 * d] * f, v[2 * d + 1] * f, hi[d], lo[d]);
-                if (bad) hi[d] = lo[d] = 0;
+                for (int d = 0; d < 4; d++) {
+                    split_pair(v[2 * d] * f, v[2 * d + 1] * f, hi[d], lo[d]);
+                    if (bad) hi[d] = lo[d] = 0;
+                }
+                if (lane == 0)
+                    reinterpret_cast<float *>(smem + kOffRowFac)[r] = bad ? __int_as_float(0x7fffffff) : power(e) * p.scale_log2;
+                const int off = sw128_offset(r, at & 63);
+                *reinterpret_cast<uint4 *>(to + off) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+                *reinterpret_cast<uint4 *>(to + (kOffK - kOffQ) + off) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
             }
-            if (lane == 0)
-                reinterpret_cast<float *>(smem + kOffRowFac)[r] = bad ? __int_as_float(0x7fffffff) : power(e) * p.scale_log2;
-            const int off = sw128_offset(r, at & 63);
-            *reinterpret_cast<uint4 *>(to + off) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
-            *reinterpret_cast<uint4 *>(to + (kOffK - kOffQ) + off) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
         }
         fence_async_shared();   // Q lo; the barriers below carry it on
         named_sync(1, 32 * kQWarps);
@@ -423,79 +417,69 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tree_tc(TreeParams p) {
             if (tid < kRows && hi_key > it.base) {
                 // which drafted rows this row sees (rows past the last: those of the last)
                 unsigned *const sees = reinterpret_cast<unsigned *>(smem + kOffSees) + tid * (kTreeWords + 1);
-                tree_ancestors(reinterpret_cast<const int *>(smem + kOffParents), (it.tile * kRows + min(tid, rows - 1)) / p.group,
+                tree_ancestors(reinterpret_cast<const int *>(smem + kOffParents), p.node_of(it.tile * kRows + min(tid, rows - 1)),
                                sees, p.status);
                 sees[kTreeWords] = 0;
             }
         }
     }
     tc_fence_before();
-    if (warp < 8 || warp == 17) named_sync(6, 9 * 32);   // Q is there (the planes are under way meanwhile)
+    if (warp < 8 || warp == 19) named_sync(6, 9 * 32);   // Q is there (the planes are under way meanwhile)
     tc_fence_after();
     const unsigned tmem = s_tmem;
 
-    if (warp == 17) {
+    if (warp == 19) {
         // ------------------------------------------------------------ MMAs
         if (n > 0) {
             constexpr unsigned kMn = 1u << 16;   // B with N contiguous
             constexpr unsigned kIdescS = idesc_f16(128, T::kKeys), kIdescO = idesc_f16(128, 64 * T::kChunks) | kMn;
             const unsigned q_lo = desc_lo_sw128(smem_u32(smem + kOffQ));
-            unsigned vc = 0;   // stages of V consumed
-            unsigned kc = 0;   // stages of K consumed
+            unsigned kc = 0, vc = 0;   // stages consumed
+            // A stage's MMAs are one straight run from one election: every instruction between two of them competes with four
+            // other warps for the scheduler (looped by fours, beside busy warps: 3,093 cycles a Q K^T, so 2,051).
+            bool ok = true;
+            auto stage = [&](unsigned bar, unsigned parity, int code) {
+                ok = __all_sync(0xffffffffu, wait(bar, parity, code));
+                tc_fence_after();
+            };
             auto qk = [&](int i) {
                 const unsigned d = tmem + kTmemS + 64 * (i & 1);
 #pragma unroll 1
                 for (int h = 0; h < T::kParts; h++, kc++) {
-                    wait(k_full + 8 * (kc % kStages), (kc / kStages) & 1, 52);
-                    __syncwarp();
-                    if (*wait.abort) return;
-                    tc_fence_after();
-                    const unsigned at = smem_u32(smem + kOffK) + (kc % kStages) * kKStage;
-                    const unsigned qh = tmem + kTmemQ + 32 * T::kChunks * h, ql = q_lo + T::kChunks * h * (kQChunk >> 4);
-                    // the small terms first: each MMA cuts the sum off, relative to what it has come to
-#pragma unroll 1
-                    for (int c = 0; c < T::kChunks; c++) {
-                        const unsigned lo = desc_lo_sw128(at + T::kPlaneBytes + c * T::kChunkBytes);
-                        if (elect_one()) {
+                    stage(k_full + 8 * (kc % kStages), (kc / kStages) & 1, 52);
+                    if (!ok) return;
+                    const unsigned hi = desc_lo_sw128(smem_u32(smem + kOffK) + (kc % kStages) * kKStage);
+                    const unsigned lo = hi + (T::kPlaneBytes >> 4), ql = q_lo + h * T::kChunks * (kQChunk >> 4);
+                    const unsigned qh = tmem + kTmemQ + 32 * T::kChunks * h, more = h != 0;
+                    if (elect_one()) {
+                        // the small terms first: each MMA cuts the sum off, relative to what it has come to
 #pragma unroll
-                            for (int k = 0; k < 4; k++)
-                                tc_mma_ts<1>(d, qh + 32 * c + 8 * k, desc_from(lo + 2 * k), kIdescS, (h | c | k) != 0);
-                        }
-                    }
-#pragma unroll 1
-                    for (int c = 0; c < T::kChunks; c++) {
-                        const unsigned hi = desc_lo_sw128(at + c * T::kChunkBytes), q = ql + c * (kQChunk >> 4);
-                        if (elect_one()) {
+                        for (int k = 0; k < 4 * T::kChunks; k++)
+                            tc_mma_ts<1>(d, qh + 8 * k, desc_from(lo + (k / 4) * (T::kChunkBytes >> 4) + 2 * (k % 4)), kIdescS,
+                                         k == 0 ? more : 1);
 #pragma unroll
-                            for (int k = 0; k < 4; k++) tc_mma_ss<1>(d, desc_from(q + 2 * k), desc_from(hi + 2 * k), kIdescS, 1);
-                        }
-                    }
-#pragma unroll 1
-                    for (int c = 0; c < T::kChunks; c++) {
-                        const unsigned hi = desc_lo_sw128(at + c * T::kChunkBytes);
-                        if (elect_one()) {
+                        for (int k = 0; k < 4 * T::kChunks; k++)
+                            tc_mma_ss<1>(d, desc_from(ql + (k / 4) * (kQChunk >> 4) + 2 * (k % 4)),
+                                         desc_from(hi + (k / 4) * (T::kChunkBytes >> 4) + 2 * (k % 4)), kIdescS, 1);
 #pragma unroll
-                            for (int k = 0; k < 4; k++) tc_mma_ts<1>(d, qh + 32 * c + 8 * k, desc_from(hi + 2 * k), kIdescS, 1);
-                        }
+                        for (int k = 0; k < 4 * T::kChunks; k++)
+                            tc_mma_ts<1>(d, qh + 8 * k, desc_from(hi + (k / 4) * (T::kChunkBytes >> 4) + 2 * (k % 4)), kIdescS, 1);
+                        tc_commit<1>(k_empty + 8 * (kc % kStages));
+                        if (h + 1 == T::kParts) tc_commit<1>(s_ready + 8 * (i & 1));
                     }
-                    if (elect_one()) tc_commit<1>(k_empty + 8 * (kc % kStages));
                     __syncwarp();
                 }
-                if (elect_one()) tc_commit<1>(s_ready + 8 * (i & 1));
-                __syncwarp();
             };
             auto pv = [&](int i) {
                 const unsigned later = (i * T::kKeys) % kFlushKeys != 0;   // 0: O starts afresh
-#pragma unroll 1
-                for (int s = 0; s < 2 * T::kParts; s++, vc++) {   // half of the rows, part of the dims
+#pragma unroll
+                for (int s = 0; s < 2 * T::kParts; s++) {   // half of the rows, part of the dims
                     const int half = s / T::kParts, h = s % T::kParts;
-                    wait(v_full + 8 * (vc % kStages), (vc / kStages) & 1, 53);
-                    __syncwarp();
-                    if (*wait.abort) return;
-                    tc_fence_after();
+                    stage(v_full + 8 * (vc % kStages), (vc / kStages) & 1, 53);
+                    if (!ok) return;
                     const unsigned a = tmem + kTmemS + 64 * (i & 1) + T::kVKeys * half, d = tmem + kTmemO + 128 * h;
-                    const unsigned at = smem_u32(smem + kOffV) + (vc % kStages) * kVStage;
-                    const unsigned hi = desc_lo_mn(at, T::kVChunkBytes), lo = desc_lo_mn(at + T::kVPlaneBytes, T::kVChunkBytes);
+                    const unsigned hi = desc_lo_mn(smem_u32(smem + kOffV) + (vc % kStages) * kVStage, T::kVChunkBytes);
+                    const unsigned lo = hi + (T::kVPlaneBytes >> 4);
                     if (elect_one()) {
 #pragma unroll
                         for (int k = 0; k < T::kVKeys / 16; k++) {   // 16 keys: two groups of eight rows
@@ -504,29 +488,25 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tree_tc(TreeParams p) {
                             tc_mma_ts<1>(d, a + 16 * k, desc_from(hi + 128 * k), kIdescO, 1);
                         }
                         tc_commit<1>(v_empty + 8 * (vc % kStages));
+                        if (s + 1 == 2 * T::kParts) tc_commit<1>(o_done + 8 * (i & 1));
                     }
                     __syncwarp();
+                    vc++;
                 }
-                if (elect_one()) tc_commit<1>(o_done + 8 * (i & 1));
-                __syncwarp();
             };
             qk(0);
-            for (int i = 0; i < n && !*wait.abort; i++) {
+            for (int i = 0; i < n && ok; i++) {
                 if (i + 1 < n) qk(i + 1);
-                if (*wait.abort) break;
-                wait(w_ready + 8 * (i & 1), (i >> 1) & 1, 54);
-                __syncwarp();
-                if (*wait.abort) break;
-                tc_fence_after();
-                pv(i);
+                if (!ok) break;
+                stage(w_ready + 8 * (i & 1), (i >> 1) & 1, 54);
+                if (ok) pv(i);
             }
-            __syncwarp();
-            if (*wait.abort) {
+            if (!ok) {
                 if (elect_one()) tc_commit<1>(all_done);
                 for (unsigned spin = 0; spin < kSpinLimit && !mbar_try_wait(all_done, 0); spin++) {}
             }
         }
-    } else if (warp == 18) {
+    } else if (warp == 17) {
         // ------------------------------------------------------------ the factors of V's rows, which the softmax wants early
         float *const value_power = reinterpret_cast<float *>(smem + kOffPow);
         float *const value_inverse = reinterpret_cast<float *>(smem + kOffInv);
@@ -552,8 +532,8 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tree_tc(TreeParams p) {
                 if constexpr (kType == 0) most = max(most, __shfl_xor_sync(0xffffffffu, most, 16));
                 bool bad;
                 const int e = row_power<kType>(most, bad);
-                value_power[64 * (t % kFactors) + key] = bad ? 0.0f : (float)(e - power0);
-                value_inverse[64 * (t % kFactors) + key] = bad ? __int_as_float(0x7fffffff) : power(power0 - e);
+                value_power[64 * (t % kFactors) + key] = bad ? __int_as_float(0x7fffffff) : (float)(e - power0);
+                value_inverse[64 * (t % kFactors) + key] = bad ? 1.0f : power(power0 - e);
                 __syncwarp();
                 if (lane == 0) mbar_arrive(raw_empty + 8 * (u % T::kRawSlots));
             }
@@ -623,6 +603,31 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tree_tc(TreeParams p) {
                 const int j = kType == 0 ? s : (is_v ? s >> 1 : s & 1), h = kType == 0 ? 0 : (is_v ? s & 1 : s >> 1);
                 const int key = T::kRawRows * j + row;
                 const unsigned full = (is_v ? v_full : k_full) + 8 * (c % kStages);
+                const float by = j ? f[1] : f[0];
+                const unsigned char *const raw_row = j ? from[1] : from[0];
+                // the block's planes in registers, before their place in shared memory is waited for
+                unsigned hi[16], lo[16];
+                if constexpr (kType == 0) {
+                    // (an odd block's halves are swapped, as above)
+                    const float4 *const src = reinterpret_cast<const float4 *>(raw_row + blk * 128);
+#pragma unroll
+                    for (int k = 0; k < 8; k++) {
+                        const float4 a = src[k ^ ((blk & 1) << 2)];
+                        split_pair(a.x * by, a.y * by, hi[2 * k], lo[2 * k]);
+                        split_pair(a.z * by, a.w * by, hi[2 * k + 1], lo[2 * k + 1]);
+                    }
+                    if (by == 0.0f) {   // (not finite, or no row at all)
+#pragma unroll
+                        for (int k = 0; k < 16; k++) hi[k] = lo[k] = 0;
+                    }
+                } else {
+                    const unsigned *const src = reinterpret_cast<const unsigned *>(raw_row) + pair * kPair + (h ? kOdd : 0);
+                    unsigned w[kOdd + 1];
+#pragma unroll
+                    for (int k = 0; k <= kOdd; k++) w[k] = src[k];
+                    const float scale = half_bits_to_float((uint16_t)(w[0] >> (16 * h)));
+                    block_planes<kType>(w, h ? 0x7654 : 0x5432, __float2half2_rn(by == 0.0f ? 0.0f : scale * by), hi, lo);
+                }
                 if (is_v || j == 0) {
                     wait((is_v ? v_empty : k_empty) + 8 * (c % kStages), ((c / kStages) & 1) ^ 1, 55);
                     if (!is_v && s == 0 && first) {
@@ -630,44 +635,17 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tree_tc(TreeParams p) {
                         for (int i = 0; i < 2; i++) key_factor[64 * (t % kFactors) + T::kRawRows * i + row] = factor[i];
                     }
                 }
-                const int chunk = kType == 0 ? blk >> 1 : pair >> 1;
-                unsigned char *const dst = is_v ? smem + kOffV + (c % kStages) * kVStage + row * 128 + chunk * T::kVChunkBytes
-                                                : smem + kOffK + (c % kStages) * kKStage + key * 128 + chunk * T::kChunkBytes;
+                const int b = kType == 0 ? blk : pair;
+                unsigned char *const dst = is_v ? smem + kOffV + (c % kStages) * kVStage + row * 128 + (b >> 1) * T::kVChunkBytes
+                                                : smem + kOffK + (c % kStages) * kKStage + key * 128 + (b >> 1) * T::kChunkBytes;
                 const int plane = is_v ? T::kVPlaneBytes : T::kPlaneBytes;
-                const float by = j ? f[1] : f[0];
-                const unsigned char *const raw_row = j ? from[1] : from[0];
-                if constexpr (kType == 0) {
-                    // (an odd block's halves are swapped, as above)
-                    const float4 *const src = reinterpret_cast<const float4 *>(raw_row + blk * 128);
 #pragma unroll
-                    for (int k = 0; k < 4; k++) {
-                        const float4 a = src[(2 * k) ^ ((blk & 1) << 2)], b = src[(2 * k + 1) ^ ((blk & 1) << 2)];
-                        const float v[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
-                        unsigned hi[4], lo[4];
-#pragma unroll
-                        for (int d = 0; d < 4; d++) {
-                            split_pair(v[2 * d] * by, v[2 * d + 1] * by, hi[d], lo[d]);
-                            if (by == 0.0f) hi[d] = lo[d] = 0;   // (not finite, or no row at all)
-                        }
-                        const int unit = 4 * (blk & 1) + (k ^ ((blk & 1) << 1));
-                        const int at = (unit ^ (key & 7)) << 4;
-                        *reinterpret_cast<uint4 *>(dst + at) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-                        *reinterpret_cast<uint4 *>(dst + plane + at) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
-                    }
-                } else {
-                    const unsigned *const src = reinterpret_cast<const unsigned *>(raw_row) + pair * kPair + (h ? kOdd : 0);
-                    unsigned w[kOdd + 1], hi[16], lo[16];
-#pragma unroll
-                    for (int k = 0; k <= kOdd; k++) w[k] = src[k];
-                    const float scale = half_bits_to_float((uint16_t)(w[0] >> (16 * h)));
-                    block_planes<kType>(w, h ? 0x7654 : 0x5432, __float2half2_rn(by == 0.0f ? 0.0f : scale * by), hi, lo);
-#pragma unroll
-                    for (int k = 0; k < 4; k++) {
-                        const int at = ((4 * (pair & 1) + k) ^ (key & 7)) << 4;
-                        *reinterpret_cast<uint4 *>(dst + at) = make_uint4(hi[4 * k], hi[4 * k + 1], hi[4 * k + 2], hi[4 * k + 3]);
-                        *reinterpret_cast<uint4 *>(dst + plane + at) =
-                            make_uint4(lo[4 * k], lo[4 * k + 1], lo[4 * k + 2], lo[4 * k + 3]);
-                    }
+                for (int k = 0; k < 4; k++) {
+                    const int unit = 4 * (b & 1) + (kType == 0 ? k ^ ((b & 1) << 1) : k);
+                    const int at = (unit ^ (key & 7)) << 4;
+                    *reinterpret_cast<uint4 *>(dst + at) = make_uint4(hi[4 * k], hi[4 * k + 1], hi[4 * k + 2], hi[4 * k + 3]);
+                    *reinterpret_cast<uint4 *>(dst + plane + at) =
+                        make_uint4(lo[4 * k], lo[4 * k + 1], lo[4 * k + 2], lo[4 * k + 3]);
                 }
                 const bool done = s + 1 == 2 * T::kParts;
                 if (is_v || j == 1) {   // the stage is written
@@ -736,8 +714,8 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tree_tc(TreeParams p) {
                 u[e + 3] = fmaf(u[e + 3] * f.w, row_factor, g.w);
             }
             const int key0 = lo_key + i * T::kKeys + T::kHalf * half;
-            unsigned sees = 0xffffffffu;
             if (lo_key + (i + 1) * T::kKeys > it.base) {   // drafted rows, and none past the last
+                unsigned sees;
                 const int from = key0 - it.base;
                 const unsigned *const words = reinterpret_cast<const unsigned *>(smem + kOffSees) + r * (kTreeWords + 1);
                 if (from <= -32) {
@@ -817,11 +795,10 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tree_tc(TreeParams p) {
             for (int e = 0; e < T::kHalf; e += 4) {
                 const float4 g = vi[e / 4];
                 const float w0 = ex2(u[e] - ref), w1 = ex2(u[e + 1] - ref), w2 = ex2(u[e + 2] - ref), w3 = ex2(u[e + 3] - ref);
-                // (a hidden row's inverse may be not a number)
-                sum[0] = sees >> e & 1 ? fmaf(w0, g.x, sum[0]) : sum[0];
-                sum[1] = sees >> (e + 1) & 1 ? fmaf(w1, g.y, sum[1]) : sum[1];
-                sum[2] = sees >> (e + 2) & 1 ? fmaf(w2, g.z, sum[2]) : sum[2];
-                sum[3] = sees >> (e + 3) & 1 ? fmaf(w3, g.w, sum[3]) : sum[3];
+                sum[0] = fmaf(w0, g.x, sum[0]);
+                sum[1] = fmaf(w1, g.y, sum[1]);
+                sum[2] = fmaf(w2, g.z, sum[2]);
+                sum[3] = fmaf(w3, g.w, sum[3]);
                 const int at = (e >> 4) * 16 + ((e & 15) >> 1);   // per 16 keys: eight words of hi, eight of lo
                 split_pair(w0, w1, o[at], o[at + 8]);
                 split_pair(w2, w3, o[at + 1], o[at + 9]);
@@ -895,7 +872,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tree_tc(TreeParams p) {
     }
     tc_fence_before();
     __syncthreads();
-    if (warp == 17) {
+    if (warp == 19) {
         tc_fence_after();
         tmem_dealloc<1>(tmem, 512);
     }

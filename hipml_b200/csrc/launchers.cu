@@ -964,6 +964,7 @@ int hipml_attn_tree(hipml_stream_t stream, int kv_dtype, const int *pos, const i
     p.n_heads = n_heads;
     p.n_kv = n_kv;
     p.group = n_heads / n_kv;
+    p.group_inverse = (65536u + p.group - 1) / p.group;
     p.head_dim = head_dim;
     p.stride = stride;
     p.nodes = nodes;

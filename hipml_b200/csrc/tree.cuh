@@ -6,8 +6,6 @@
 
 namespace hipml {
 
-__host__ __device__ __forceinline__ int div_up_int(int a, int b) { return (a + b - 1) / b; }
-
 constexpr int kTreeNodes = 256;                      // most nodes of a slot's tree
 constexpr int kTreeWords = kTreeNodes / 32;
 constexpr int kTreeKeyTile = 64;                     // cache rows that runs are counted in
@@ -31,6 +29,9 @@ struct TreeParams {
     float scale_log2;
     size_t slot_bytes;
     int grid, tile_rows;
+    unsigned group_inverse;   // 65536 / group, rounded up
+    // row / group, of the rows of a slot (fewer than 65536 / 8)
+    __device__ __forceinline__ int node_of(int row) const { return (int)((unsigned)row * group_inverse >> 16); }
 };
 
 // Prefix rows and live nodes of a slot; whatever `pos` says, no row lies past the cache and no node past `nodes`.
@@ -65,6 +66,8 @@ struct TreeItem {
 };
 
 // The slots as a warp's lanes hold them: the first 32 stay in registers, so that the plan is one trip to memory.
+// kRows: rows of a tile.
+template <int kRows>
 struct TreeSlots {
     const TreeParams &p;
     TreeSlot mine;
@@ -75,72 +78,87 @@ struct TreeSlots {
     __device__ __forceinline__ TreeSlot at(int s) const {   // s % 32 == lane
         return s < 32 ? mine : tree_slot(p.pos, s, p.stride, p.nodes);
     }
+    static __device__ __forceinline__ unsigned keys(const TreeSlot &t) {   // key tiles
+        return (unsigned)(t.base + t.live + kTreeKeyTile - 1) / kTreeKeyTile;
+    }
+    __device__ __forceinline__ unsigned tiles(const TreeSlot &t) const {   // of rows
+        return (unsigned)(t.live * p.group + kRows - 1) / kRows;
+    }
 };
 
-// Key tiles per run, the same for all: the fewest with which the runs fit the grid. Called by a whole warp.
-__device__ __forceinline__ int tree_quota(const TreeParams &p, const TreeSlots &slots) {
+// Key tiles per run, the same for all: the fewest with which the runs fit the grid. Called by a whole warp. (One loop over
+// the slots: this runs once, and every line of it comes through an empty instruction cache.)
+template <int kRows>
+__device__ __forceinline__ int tree_quota(const TreeParams &p, const TreeSlots<kRows> &slots) {
     const int lane = threadIdx.x & 31;
-    auto each = [&](auto f) {   // sum over the slots of f(key tiles, row tiles)
-        int n = 0;
+    const unsigned fit = (unsigned)p.grid / (unsigned)p.n_kv;   // runs per KV head
+    // question 0: the tiles of all; then the runs that quota q makes
+    unsigned lo = 1, hi = 0, q = 1;
+#pragma unroll 1
+    for (int asked = 0;; asked++) {
+        unsigned runs = 0, rows = 0;
+#pragma unroll 1
         for (int s = lane; s < p.slots; s += 32) {
             const TreeSlot t = slots.at(s);
-            n += f(div_up_int(t.base + t.live, kTreeKeyTile), div_up_int(t.live * p.group, p.tile_rows));
+            const unsigned r = slots.tiles(t);
+            runs += r * ((slots.keys(t) + q - 1) / q);
+            rows += r;
         }
-        return (int)__reduce_add_sync(0xffffffffu, n);
-    };
-    const int fit = p.grid / p.n_kv;   // runs per KV head
-    const int total = each([](int keys, int rows) { return keys * rows; });
-    auto runs_at = [&](int q) { return each([&](int keys, int rows) { return rows * div_up_int(keys, q); }); };
-    int lo = max(1, div_up_int(total, fit));
-    if (runs_at(lo) <= fit) return lo;
-    // sum(rows * ceil(keys / q)) <= total / q + few; with one run each, every triple has its CTA
-    const int few = each([](int, int rows) { return rows; });
-    int hi = fit > few ? div_up_int(total, fit - few) : div_up_int(p.stride, kTreeKeyTile);
-    hi = max(hi, lo + 1);
-    while (hi - lo > 1) {
-        const int mid = lo + (hi - lo) / 2;
-        if (runs_at(mid) <= fit) hi = mid; else lo = mid;
+        runs = __reduce_add_sync(0xffffffffu, runs);
+        if (asked == 0) {   // (q was 1)
+            rows = __reduce_add_sync(0xffffffffu, rows);
+            if (runs <= fit) return 1;
+            lo = (runs + fit - 1) / fit;
+            // sum(rows * ceil(keys / q)) <= runs / q + rows; with one run each, every triple has its CTA
+            hi = fit > rows ? (runs + fit - rows - 1) / (fit - rows) : (unsigned)(p.stride + kTreeKeyTile - 1) / kTreeKeyTile;
+            q = lo;
+            lo--;       // (does not fit; hi does)
+            if (hi <= q) return (int)q;
+            continue;
+        }
+        if (runs <= fit) hi = q; else lo = q;
+        if (hi - lo <= 1) return (int)hi;
+        q = asked == 1 ? q + 1 : lo + (hi - lo) / 2;   // (most often the least that may do, or the next, does)
+        if (q >= hi) q = lo + (hi - lo) / 2;
     }
-    return hi;
-}
-
-__device__ __forceinline__ int tree_ctas(const TreeParams &p, const TreeSlot &t, int quota) {
-    return p.n_kv * div_up_int(t.live * p.group, p.tile_rows) * div_up_int(t.base + t.live, kTreeKeyTile * quota);
 }
 
 // CTA `cta`'s item (slot < 0: none); a slot's first CTA leaves its share for the fold. Called by a whole warp.
+template <int kRows>
 __device__ __forceinline__ TreeItem tree_item(const TreeParams &p, int cta) {
     const int lane = threadIdx.x & 31;
-    const TreeSlots slots(p);
-    const int quota = tree_quota(p, slots);
+    const TreeSlots<kRows> slots(p);
+    const int quota = tree_quota<kRows>(p, slots);
     TreeItem it;
     it.slot = -1;
     it.quota = quota;
-    int before = 0;
+    unsigned before = 0;
+#pragma unroll 1
     for (int s0 = 0; s0 < p.slots && it.slot < 0; s0 += 32) {
         TreeSlot t = {0, 0};
         if (s0 + lane < p.slots) t = slots.at(s0 + lane);
-        const int mine = tree_ctas(p, t, quota);
-        int upto = mine;
-#pragma unroll
+        const unsigned tiles = slots.tiles(t), runs = (slots.keys(t) + quota - 1) / (unsigned)quota;
+        const unsigned mine = p.n_kv * tiles * runs;
+        unsigned upto = mine;
+#pragma unroll 1
         for (int o = 1; o < 32; o <<= 1) {
-            const int x = __shfl_up_sync(0xffffffffu, upto, o);
+            const unsigned x = __shfl_up_sync(0xffffffffu, upto, o);
             if (lane >= o) upto += x;
         }
-        const unsigned past = __ballot_sync(0xffffffffu, cta < before + upto);
+        const unsigned past = __ballot_sync(0xffffffffu, (unsigned)cta < before + upto);
         if (past) {
             const int at = __ffs(past) - 1;
-            const int first = before + __shfl_sync(0xffffffffu, upto - mine, at);
+            const unsigned first = before + __shfl_sync(0xffffffffu, upto - mine, at);
             it.slot = s0 + at;
             it.base = __shfl_sync(0xffffffffu, t.base, at);
             it.live = __shfl_sync(0xffffffffu, t.live, at);
-            it.runs = div_up_int(it.base + it.live, kTreeKeyTile * quota);
-            const int in_slot = cta - first, tiles = div_up_int(it.live * p.group, p.tile_rows);
-            const int triple = in_slot / it.runs;
-            it.run = in_slot - triple * it.runs;
-            it.kvh = triple / tiles;
-            it.tile = triple - it.kvh * tiles;
-            if (in_slot == 0 && lane == 0) p.shares[it.slot] = make_int4(cta, it.runs, tiles, 0);
+            it.runs = (int)__shfl_sync(0xffffffffu, runs, at);
+            const unsigned of_slot = __shfl_sync(0xffffffffu, tiles, at), in_slot = cta - first;
+            const unsigned triple = in_slot / (unsigned)it.runs;
+            it.run = (int)(in_slot - triple * it.runs);
+            it.kvh = (int)(triple / of_slot);
+            it.tile = (int)(triple - it.kvh * of_slot);
+            if (in_slot == 0 && lane == 0) p.shares[it.slot] = make_int4(cta, it.runs, (int)of_slot, 0);
         }
         before += __shfl_sync(0xffffffffu, upto, 31);
     }
@@ -150,7 +168,9 @@ __device__ __forceinline__ TreeItem tree_item(const TreeParams &p, int cta) {
 // Bits of the drafted rows that `node` sees, its own and those of its ancestors, into words[kTreeWords]. A parent that is no
 // earlier node ends the walk (and is reported).
 __device__ __forceinline__ void tree_ancestors(const int *parents, int node, unsigned *words, int *status) {
+#pragma unroll 1
     for (int w = 0; w < kTreeWords; w++) words[w] = 0;
+#pragma unroll 1
     for (int i = node; i >= 0;) {
         words[i >> 5] |= 1u << (i & 31);
         const int up = parents[i];
