@@ -13,11 +13,12 @@
 // dims contiguous along K, for V the same image with them along N. A q8_0 or q4_0 value (11-bit scale times a code of 8
 // bits) is exactly hi + lo: hi is its f16 product and lo the f16 FMA's remainder, two instructions for two values.
 //
-// f16 parts need their operands in range whatever the cache holds. So each key and each value row is scaled by a power of two
-// of its own, by its largest scale (f32: value), and each query row too. S is multiplied back (a factor per key and one
-// per row); the value's power 2^E goes into the weight: w = 2^(s + E - m), where m follows the largest s + E, and the
-// denominator takes w 2^-E. A row that is not finite is zero in the planes and its factor (or power) is not a number, so it
-// reaches the rows that see it and no others (a hidden key's weight is 0, and 0 times its plane is 0).
+// f16 parts need their operands in range whatever the cache holds. So the rows of a tile are scaled by a power of two, K's
+// and V's each by its largest scale (f32: value), and each query row by one of its own. S is multiplied back; the value's
+// power 2^E goes into the weight: w = 2^(s + E - m), where m follows the largest s + E, and the denominator takes w 2^-E.
+// (A row far smaller than its tile's largest has fewer bits: 22 of them down to 2^-10 of it, one fewer for each power below.)
+// A K row that is not finite is not a number in the planes, which reaches the rows that see it and no others; a V row that is
+// not finite is zero there, and the weights of those that see it are not a number (a hidden key's weight is 0).
 //
 // Where the time goes (a quantised tile of 64 rows): tensor pipe 2 x 1,536 cycles; shared memory 7.1 KB a row: the raw
 // bytes in and out (1.1), the planes (2), K and the low part of Q into the pipe (2.5), V (1.5), 55 cycles a row at 128
@@ -53,11 +54,11 @@ constexpr int kQBytes = 4 * kQChunk;             // one plane of Q
 constexpr int kStages = 2;                       // of K and of V
 constexpr int kKStage = 32 * 1024, kVStage = 16 * 1024;
 constexpr int kRawBytes = 3 * 64 * 272;
-constexpr int kFlushKeys = 1024;
+constexpr int kFlushKeys = 512;
 constexpr unsigned kSpinLimit = 1u << 22;
 constexpr float kThreshold = 8.0f;               // log2: the reference moves when a weight would exceed 2^8 times it,
 constexpr float kLift = 7.0f;                    // and weights are kept 2^7 times larger: below 2^15, f16's smallest 2^-24
-constexpr int kLeastPower = -100, kMostPower = 100;   // of a key or value row; smaller values count as 0 (as do rows of zeros)
+constexpr int kLeastPower = -100, kMostPower = 100;   // of a tile; smaller values count as 0 (as do zeros)
 
 template <int kType>   // 0 f32, 1 q8_0, 2 q4_0
 struct Shape {
@@ -86,20 +87,21 @@ constexpr int kOffQ = 0;                                   // Q lo
 constexpr int kOffK = kOffQ + kQBytes;
 constexpr int kOffV = kOffK + kStages * kKStage;
 constexpr int kOffRaw = kOffV + kStages * kVStage;
-// A tile's factors of K are written once its planes have their stage, those of V once its rows are in the ring. By then the
-// tile four before has been through the softmax: W V of tile t - 4 was issued before Q K^T of t - 2, which had to be done
-// for the stage to be free, and the slot of the ring that V's rows take was free at the earliest when planes were made that
-// needed the same.
-constexpr int kFactors = 4;
-constexpr int kOffKey = kOffRaw + kRawBytes;               // [kFactors][64] factor of S, by key
-constexpr int kOffPow = kOffKey + kFactors * 64 * 4;       // [kFactors][64] E
-constexpr int kOffInv = kOffPow + kFactors * 64 * 4;       // [kFactors][64] 2^-E
-constexpr int kOffMeet = kOffInv + kFactors * 64 * 4;      // [2][2][128]: the halves of a row meet
+// What is known of a tile's rows ahead of their planes: the power of two of K, that of V, and which rows are not finite. A
+// ring of eight tiles: a tile's rows are in the raw ring at the earliest when planes were made that needed Q K^T of three
+// tiles before, and that came after the softmax of two more.
+constexpr int kScouts = 8;
+struct __align__(16) Scout {
+    int power;
+    unsigned bad[2];   // a bit per row
+};
+constexpr int kOffScout = kOffRaw + kRawBytes;             // [K, V][kScouts]
+constexpr int kOffMeet = kOffScout + 2 * kScouts * 16;      // [2][2][128]: the halves of a row meet
 constexpr int kOffRowFac = kOffMeet + 2 * 2 * 128 * 4;     // [128]
 constexpr int kOffSees = kOffRowFac + kRows * 4;           // [128][kTreeWords + 1]
 constexpr int kOffParents = kOffSees + kRows * (kTreeWords + 1) * 4;
 constexpr int kOffBars = kOffParents + kTreeNodes * 4;
-constexpr int kBars = 43;
+constexpr int kBars = 55;
 constexpr int kSmemNeed = kOffBars + kBars * 8;
 constexpr int kSmemBytes = (kSmemNeed + 15) / 16 * 16 + 1024;               // (the planes lie on 1 KB boundaries)
 static_assert(kSmemBytes <= 227 * 1024, "one CTA per SM");
@@ -162,15 +164,6 @@ __device__ __forceinline__ void split_pair(float a, float b, unsigned &hi, unsig
 // 2^n for whole n of [-126, 127]
 __device__ __forceinline__ float power(int n) { return __int_as_float((n + 127) << 23); }
 
-// The power of two that brings a row into range, from its largest |value| (f32: its bits) or |scale| (its bits): values come
-// to [2^10, 2^11), scales to [8, 16), so that codes times them stay below 2^11 and lo is exact.
-template <int kType>
-__device__ __forceinline__ int row_power(unsigned most, bool &bad) {
-    bad = most >= (kType == 0 ? 0x7f800000u : 0x7c00u);
-    if (bad) return 0;
-    if (kType == 0) return min(max((int)(most >> 23) - 127 - 10, kLeastPower), kMostPower);
-    return most == 0 ? kLeastPower : max((int)most >> 10, 1) - 15 - 3;
-}
 // The largest |value| of half of an f32 row, or |scale| of a quantised row, as bits.
 template <int kType>
 __device__ __forceinline__ unsigned row_most(const unsigned char *row, int half) {
@@ -188,27 +181,12 @@ __device__ __forceinline__ unsigned row_most(const unsigned char *row, int half)
     }
     return most;
 }
-
-// The power of two of a value row in shared memory, clamped: by a whole warp.
+// The power of two that brings rows into range, from their largest |value| or |scale| as bits: values come to [2^10, 2^11),
+// scales to [8, 16), so that codes times them stay below 2^11 and lo is exact.
 template <int kType>
-__device__ __forceinline__ int first_power(const unsigned char *row, int lane) {
-    int top;
-    if constexpr (kType == 0) {
-        const uint4 *const src = reinterpret_cast<const uint4 *>(row) + 2 * lane;
-        unsigned most = 0;
-#pragma unroll
-        for (int k = 0; k < 2; k++) {
-            const uint4 x = src[k];
-            most = max(max(most, x.x & 0x7fffffffu), max(max(x.y & 0x7fffffffu, x.z & 0x7fffffffu), x.w & 0x7fffffffu));
-        }
-        most = __reduce_max_sync(0xffffffffu, most);
-        top = most > 0 ? (int)(most >> 23) - 127 - 10 : 0;
-    } else {
-        const unsigned short scale = *reinterpret_cast<const unsigned short *>(row + (lane & 7) * (kType == 1 ? 34 : 18));
-        const int most = __reduce_max_sync(0xffffffffu, (int)(scale & 0x7fff));
-        top = most > 0 ? max(most >> 10, 1) - 15 - 3 : 0;
-    }
-    return min(max(top, -20), 16);
+__device__ __forceinline__ int power_of(unsigned most) {
+    if (kType == 0) return min(max((int)(most >> 23) - 127 - 10, kLeastPower), kMostPower);
+    return most == 0 ? kLeastPower : max((int)most >> 10, 1) - 15 - 3;
 }
 
 // A quantised block's 32 values times scale, as hi and lo words in the order of the dims. `w`: its words from the one that
@@ -247,7 +225,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tree_tc(TreeParams p) {
     unsigned char *const smem =
         reinterpret_cast<unsigned char *>((reinterpret_cast<size_t>(smem_raw) + 1023) & ~(size_t)1023);
     __shared__ TreeItem s_item;
-    __shared__ int s_abort, s_power0;
+    __shared__ int s_abort;
     __shared__ unsigned s_tmem;
     griddep_launch();
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -257,17 +235,19 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tree_tc(TreeParams p) {
     const unsigned raw_full = smem_u32(bars), raw_empty = smem_u32(bars + 16), k_full = smem_u32(bars + 24),
                    k_empty = smem_u32(bars + 26), v_full = smem_u32(bars + 28), v_empty = smem_u32(bars + 30),
                    s_ready = smem_u32(bars + 32), w_ready = smem_u32(bars + 34), o_done = smem_u32(bars + 36),
-                   factors = smem_u32(bars + 38), all_done = smem_u32(bars + 42);
-    static_assert(T::kRawSlots <= 8 && kFactors <= 4 && kBars == 43, "barriers");
+                   scouted = smem_u32(bars + 38), all_done = smem_u32(bars + 54);
+    static_assert(T::kRawSlots <= 8 && kScouts == 8 && kBars == 55, "barriers");
+    auto scout_bar = [&](bool v, int t) { return scouted + 8 * ((v ? 8 : 0) + (t & 7)); };   // of tile t
+    Scout *const scouts = reinterpret_cast<Scout *>(smem + kOffScout);
     auto raw_bar = [&](bool v, int i) { return raw_full + 8 * ((v ? 8 : 0) + (i & 7)); };   // of half tile i
     if (warp == 1) {
-        // four warps make planes of a raw slot's rows; warp 17 reads V's as well (and K's first warp arrives once more)
         for (int i = lane; i < kBars; i += 32) {
-            const int kind = i / 2;   // from 12 on: pairs of k_full, k_empty, v_full, v_empty, s_ready, w_ready, o_done
-            mbar_init(raw_full + 8 * i, i < 16 ? 1 : i < 24 || (i >= 38 && i < 42) ? kGroup + 1
-                                                   : kind == 12 || kind == 14    ? kGroup
-                                                   : kind == 17                  ? 8
-                                                                                 : 1);
+            const int pair = i / 2;   // from 12 on: k_full, k_empty, v_full, v_empty, s_ready, w_ready, o_done
+            // (a raw slot is read by four warps that make planes and one that scouts)
+            mbar_init(raw_full + 8 * i, i >= 16 && i < 24          ? kGroup + 1
+                                        : pair == 12 || pair == 14 ? kGroup
+                                        : pair == 17               ? 8
+                                                                   : 1);
         }
         if (lane == 0) s_abort = 0;
         mbar_init_fence();
@@ -380,7 +360,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tree_tc(TreeParams p) {
                 const bool bad = most >= 0x7f800000u;
                 // the row's largest value comes to [2^10, 2^11)
                 const int e = min(max((int)(most >> 23) - 127 - 10, -116), 116);
-                const float f = power(-e);
+                const float f = copysignf(power(-e), p.scale_log2);   // (the largest score is the largest S)
                 unsigned hi[4], lo[4];
 #pragma unroll
                 for (int d = 0; d < 4; d++) {
@@ -388,7 +368,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tree_tc(TreeParams p) {
                     if (bad) hi[d] = lo[d] = 0;
                 }
                 if (lane == 0)
-                    reinterpret_cast<float *>(smem + kOffRowFac)[r] = bad ? __int_as_float(0x7fffffff) : power(e) * p.scale_log2;
+                    reinterpret_cast<float *>(smem + kOffRowFac)[r] = bad ? __int_as_float(0x7fffffff) : power(e) * fabsf(p.scale_log2);
                 const int off = sw128_offset(r, at & 63);
                 *reinterpret_cast<uint4 *>(to + off) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
                 *reinterpret_cast<uint4 *>(to + (kOffK - kOffQ) + off) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
@@ -506,76 +486,50 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tree_tc(TreeParams p) {
                 for (unsigned spin = 0; spin < kSpinLimit && !mbar_try_wait(all_done, 0); spin++) {}
             }
         }
-    } else if (warp == 17) {
-        // ------------------------------------------------------------ the factors of V's rows, which the softmax wants early
-        float *const value_power = reinterpret_cast<float *>(smem + kOffPow);
-        float *const value_inverse = reinterpret_cast<float *>(smem + kOffInv);
-        // Values' powers are taken relative to that of the run's first row: the exponents of the weights stay as small as
-        // the scores, to whose rounding they would add. (Within [-20, 16], which keeps the differences in range.)
-        int power0 = 0;
+    } else if (warp == 17 || warp == 18) {
+        // ------------------------------------------------------------ scouts: warp 17 of V, 18 of K
+        const bool is_v = warp == 17;
 #pragma unroll 1
         for (int t = 0; t < n; t++) {
             const int live = tile_rows(t);
+            Scout found = {0, {0, 0}};
+            unsigned most = 0;   // of the rows that are finite
 #pragma unroll 1
             for (int j = 0; j < 2; j++) {
-                const unsigned u = raw_of(true, t) + j;
-                wait(raw_bar(true, 2 * t + j), ((2 * t + j) >> 3) & 1, 56);
+                const unsigned u = raw_of(is_v, t) + j;
+                wait(raw_bar(is_v, 2 * t + j), ((2 * t + j) >> 3) & 1, 56);
                 const unsigned char *const from = smem + kOffRaw + (u % T::kRawSlots) * T::kRawSlot;
-                if (t == 0 && j == 0) {
-                    power0 = first_power<kType>(from, lane);
-                    if (lane == 0) s_power0 = power0;
-                }
                 // f32: a lane has half of a row; quantised: a lane has a row
-                const int r = kType == 0 ? lane & 15 : lane, key = T::kRawRows * j + r;
-                unsigned most = 0;
-                if (key < live) most = row_most<kType>(from + r * T::kRowPitch, kType == 0 ? lane >> 4 : 0);
-                if constexpr (kType == 0) most = max(most, __shfl_xor_sync(0xffffffffu, most, 16));
-                bool bad;
-                const int e = row_power<kType>(most, bad);
-                value_power[64 * (t % kFactors) + key] = bad ? __int_as_float(0x7fffffff) : (float)(e - power0);
-                value_inverse[64 * (t % kFactors) + key] = bad ? 1.0f : power(power0 - e);
-                __syncwarp();
+                const int r = kType == 0 ? lane & 15 : lane;
+                unsigned mine = 0;
+                if (T::kRawRows * j + r < live) mine = row_most<kType>(from + r * T::kRowPitch, kType == 0 ? lane >> 4 : 0);
+                if constexpr (kType == 0) mine = max(mine, __shfl_xor_sync(0xffffffffu, mine, 16));
+                const bool bad = mine >= (kType == 0 ? 0x7f800000u : 0x7c00u);
+                const unsigned bits = __ballot_sync(0xffffffffu, bad);
+                if (kType == 0)
+                    found.bad[0] |= (bits & 0xffff) << (16 * j);
+                else
+                    found.bad[j] = bits;
+                if (!bad) most = max(most, mine);
                 if (lane == 0) mbar_arrive(raw_empty + 8 * (u % T::kRawSlots));
             }
-            if (lane == 0) mbar_arrive(factors + 8 * (t % kFactors));
+            found.power = power_of<kType>(__reduce_max_sync(0xffffffffu, most));
+            if (lane == 0) {
+                scouts[(is_v ? kScouts : 0) + (t & 7)] = found;
+                mbar_arrive(scout_bar(is_v, t));
+            }
         }
     } else if (warp >= 8 && warp < 16) {
         // ------------------------------------------------------------ planes: warps 8-11 of K, 12-15 of V
         const bool is_v = warp >= 12;
         const int w4 = warp & 3;
-        float *const key_factor = reinterpret_cast<float *>(smem + kOffKey);
-        // half tile i of this kind, in raw slot u: waits until it is there
-        auto raw = [&](int i, unsigned u) {
-            wait(raw_bar(is_v, i), (i >> 3) & 1, 56);
-            return smem + kOffRaw + (u % T::kRawSlots) * T::kRawSlot;
-        };
-        auto free_raw = [&](unsigned u, int times) {
-            __syncwarp();
-            if (lane == 0)
-                for (int i = 0; i < times; i++) mbar_arrive(raw_empty + 8 * (u % T::kRawSlots));
-        };
         constexpr int kPair = kType == 1 ? 17 : 9, kOdd = kType == 1 ? 8 : 4;   // words of two blocks; the odd block's first
         // Thread's row of half tile j. f32: block lane / 4 of row 4 (warp % 4) + lane % 4 (of 16). Quantised: pair lane / 8 of
         // row 8 (warp % 4) + lane % 8 (of 32), one block of it in each part.
         const int row = kType == 0 ? 4 * w4 + (lane & 3) : 8 * w4 + (lane & 7);
         const int blk = lane >> 2, pair = lane >> 3;
-        const bool first = (kType == 0 ? blk : pair) == 0;   // the lane that speaks for a row
-        // the largest of the thread's part of a row
-        auto most_of = [&](const unsigned char *from, bool live) {
-            unsigned m = 0;
-            if (!live) return m;
-            if constexpr (kType == 0) {
-                const uint4 *const src = reinterpret_cast<const uint4 *>(from + blk * 128);
-#pragma unroll
-                for (int k = 0; k < 8; k++) {
-                    const uint4 x = src[k ^ ((blk & 1) << 2)];   // (eight lanes' words fall into different banks)
-                    m = max(max(m, x.x & 0x7fffffffu), max(max(x.y & 0x7fffffffu, x.z & 0x7fffffffu), x.w & 0x7fffffffu));
-                }
-            } else {
-                const unsigned *const src = reinterpret_cast<const unsigned *>(from) + pair * kPair;
-                m = max(src[0] & 0x7fffu, (src[kOdd] >> 16) & 0x7fffu);
-            }
-            return m;
+        auto free_raw = [&](unsigned u) {
+            if (lane == 0) mbar_arrive(raw_empty + 8 * (u % T::kRawSlots));
         };
         if (!is_v && n > 0) named_sync(7, 12 * 32);   // Q hi has left K's stages
         unsigned c = 0;                               // stages written
@@ -583,32 +537,23 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tree_tc(TreeParams p) {
         for (int t = 0; t < n; t++) {
             const int live = tile_rows(t);
             const unsigned u0 = raw_of(is_v, t);   // the tile's first raw slot
-            const unsigned char *from[2];
-            float f[2], factor[2];
-#pragma unroll
-            for (int j = 0; j < 2; j++) {
-                const int key = T::kRawRows * j + row;
-                from[j] = raw(2 * t + j, u0 + j) + row * T::kRowPitch;
-                unsigned most = most_of(from[j], key < live);
-#pragma unroll
-                for (int o = kType == 0 ? 4 : 8; o < 32; o <<= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
-                bool bad;
-                const int e = row_power<kType>(most, bad);
-                f[j] = bad || (kType != 0 && e == kLeastPower) || key >= live ? 0.0f : power(-e);
-                factor[j] = bad ? __int_as_float(0x7fffffff) : power(e);
-            }
+            wait(raw_bar(is_v, 2 * t), ((2 * t) >> 3) & 1, 56);
+            wait(raw_bar(is_v, 2 * t + 1), ((2 * t + 1) >> 3) & 1, 56);
+            wait(scout_bar(is_v, t), (t >> 3) & 1, 58);
+            const Scout known = scouts[(is_v ? kScouts : 0) + (t & 7)];
+            const float scale_by = power(-known.power);
             // K: both halves of a part, then the other part; V: both parts of a half, then the other half
 #pragma unroll 1
             for (int s = 0; s < 2 * T::kParts; s++) {
                 const int j = kType == 0 ? s : (is_v ? s >> 1 : s & 1), h = kType == 0 ? 0 : (is_v ? s & 1 : s >> 1);
                 const int key = T::kRawRows * j + row;
                 const unsigned full = (is_v ? v_full : k_full) + 8 * (c % kStages);
-                const float by = j ? f[1] : f[0];
-                const unsigned char *const raw_row = j ? from[1] : from[0];
-                // the block's planes in registers, before their place in shared memory is waited for
+                const unsigned char *const raw_row = smem + kOffRaw + ((u0 + j) % T::kRawSlots) * T::kRawSlot + row * T::kRowPitch;
+                const bool bad = (key < 32 ? known.bad[0] : known.bad[1]) >> (key & 31) & 1;
+                const float by = key < live && !bad ? scale_by : 0.0f;
                 unsigned hi[16], lo[16];
                 if constexpr (kType == 0) {
-                    // (an odd block's halves are swapped, as above)
+                    // (an odd block's halves are swapped: eight lanes' words fall into different banks)
                     const float4 *const src = reinterpret_cast<const float4 *>(raw_row + blk * 128);
 #pragma unroll
                     for (int k = 0; k < 8; k++) {
@@ -616,7 +561,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tree_tc(TreeParams p) {
                         split_pair(a.x * by, a.y * by, hi[2 * k], lo[2 * k]);
                         split_pair(a.z * by, a.w * by, hi[2 * k + 1], lo[2 * k + 1]);
                     }
-                    if (by == 0.0f) {   // (not finite, or no row at all)
+                    if (by == 0.0f) {   // (not finite, or no row at all: there may be anything)
 #pragma unroll
                         for (int k = 0; k < 16; k++) hi[k] = lo[k] = 0;
                     }
@@ -628,13 +573,8 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tree_tc(TreeParams p) {
                     const float scale = half_bits_to_float((uint16_t)(w[0] >> (16 * h)));
                     block_planes<kType>(w, h ? 0x7654 : 0x5432, __float2half2_rn(by == 0.0f ? 0.0f : scale * by), hi, lo);
                 }
-                if (is_v || j == 0) {
-                    wait((is_v ? v_empty : k_empty) + 8 * (c % kStages), ((c / kStages) & 1) ^ 1, 55);
-                    if (!is_v && s == 0 && first) {
-#pragma unroll
-                        for (int i = 0; i < 2; i++) key_factor[64 * (t % kFactors) + T::kRawRows * i + row] = factor[i];
-                    }
-                }
+                if (bad && !is_v) hi[0] = 0x7fff7fff;   // one value is enough: the row's scores are not a number
+                if (is_v || j == 0) wait((is_v ? v_empty : k_empty) + 8 * (c % kStages), ((c / kStages) & 1) ^ 1, 55);
                 const int b = kType == 0 ? blk : pair;
                 unsigned char *const dst = is_v ? smem + kOffV + (c % kStages) * kVStage + row * 128 + (b >> 1) * T::kVChunkBytes
                                                 : smem + kOffK + (c % kStages) * kKStage + key * 128 + (b >> 1) * T::kChunkBytes;
@@ -651,15 +591,19 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tree_tc(TreeParams p) {
                 if (is_v || j == 1) {   // the stage is written
                     fence_async_shared();
                     __syncwarp();
-                    if (lane == 0) {
-                        mbar_arrive(full);
-                        if (!is_v && done) mbar_arrive(factors + 8 * (t % kFactors));
-                    }
+                    if (lane == 0) mbar_arrive(full);
                     c++;
                 }
                 // a half's rows were read for the last time
-                if (done || (is_v && T::kParts == 2 && s == 1) || (kType == 0)) free_raw(u0 + j, warp == 8 ? 2 : 1);
-                if (!is_v && T::kParts == 2 && done) free_raw(u0, warp == 8 ? 2 : 1);
+                if (kType == 0) {
+                    __syncwarp();
+                    free_raw(u0 + j);
+                } else if (is_v) {
+                    if (h == 1) free_raw(u0 + j);
+                } else if (done) {
+                    free_raw(u0);
+                    free_raw(u0 + 1);
+                }
             }
         }
     } else if (warp < 8 && n > 0) {
@@ -668,8 +612,6 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tree_tc(TreeParams p) {
         const unsigned lane_at = tmem + ((unsigned)((warp & 3) * 32) << 16);
         const float row_factor = reinterpret_cast<const float *>(smem + kOffRowFac)[r];
         const bool live = r < rows, whole = it.runs == 1;
-        float *const dst = (whole ? p.out + head_row(min(r, rows - 1)) * kD
-                                  : p.part_acc + ((size_t)blockIdx.x * kRows + r) * kD);
         float m = -INFINITY, l = 0.0f, m_out = -INFINITY;   // m_out: the reference of what is in memory already
         // the other half's value of the row (the warps w and w + 4 meet)
         auto meet = [&](int x, float mine) {
@@ -681,6 +623,10 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tree_tc(TreeParams p) {
         // dims of column group j (32 columns) of this thread's half of O
         auto dims_of = [&](int j) { return kType == 0 ? 128 * half + 32 * j : 32 * T::block(half, j); };
         const bool idle = 32 * (warp & 3) >= rows;   // (no row of this warp is live: nothing reads its lanes)
+        // Values' powers are taken relative to that of the run's first tile: the exponents of the weights stay as small as
+        // the scores, to whose rounding they would add. (Within [-20, 16], which keeps the differences in range.)
+        int power0 = 0;
+        float *const flushed = p.part_acc + ((size_t)blockIdx.x * kRows * (kD / 4) + r) * 4;   // [64 x four dims][128 rows]
 #pragma unroll 1
         for (int i = 0; i < n; i++) {
             const unsigned s_at = lane_at + kTmemS + 64 * (i & 1) + T::kHalf * half;
@@ -690,7 +636,13 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tree_tc(TreeParams p) {
                 if (lane == 0) mbar_arrive(w_ready + 8 * (i & 1));
                 continue;
             }
-            wait(factors + 8 * (i % kFactors), (i / kFactors) & 1, 58);
+            wait(scout_bar(false, i), (i >> 3) & 1, 58);
+            wait(scout_bar(true, i), (i >> 3) & 1, 58);
+            const Scout known = scouts[kScouts + (i & 7)];
+            if (i == 0) power0 = min(max(known.power, -20), 16);
+            const float value_power = (float)(known.power - power0), value_inverse = power(power0 - known.power);
+            float factor = row_factor * power(scouts[i & 7].power);   // of S; > 0, so that a hidden row's -inf stays that
+            if (factor < 1e-30f) factor = 1e-30f;
             __syncwarp();
             tc_fence_after();
             float u[T::kHalf];
@@ -702,18 +654,13 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tree_tc(TreeParams p) {
             } else {
                 tmem_ld16(s_at, u);
             }
-            const float4 *const kf = reinterpret_cast<const float4 *>(smem + kOffKey) + 16 * (i % kFactors) + T::kHalf / 4 * half;
-            const float4 *const vp = reinterpret_cast<const float4 *>(smem + kOffPow) + 16 * (i % kFactors) + T::kHalf / 4 * half;
-            const float4 *const vi = reinterpret_cast<const float4 *>(smem + kOffInv) + 16 * (i % kFactors) + T::kHalf / 4 * half;
-#pragma unroll
-            for (int e = 0; e < T::kHalf; e += 4) {
-                const float4 f = kf[e / 4], g = vp[e / 4];
-                u[e] = fmaf(u[e] * f.x, row_factor, g.x);
-                u[e + 1] = fmaf(u[e + 1] * f.y, row_factor, g.y);
-                u[e + 2] = fmaf(u[e + 2] * f.z, row_factor, g.z);
-                u[e + 3] = fmaf(u[e + 3] * f.w, row_factor, g.w);
-            }
             const int key0 = lo_key + i * T::kKeys + T::kHalf * half;
+            if ((known.bad[0] | known.bad[1]) != 0) {   // rare: a V row that is not finite
+                const unsigned bits = T::kHalf == 32 ? known.bad[half] : known.bad[0] >> (16 * half);
+#pragma unroll
+                for (int e = 0; e < T::kHalf; e++)
+                    if (bits >> e & 1) u[e] = __int_as_float(0x7fffffff);
+            }
             if (lo_key + (i + 1) * T::kKeys > it.base) {   // drafted rows, and none past the last
                 unsigned sees;
                 const int from = key0 - it.base;
@@ -737,7 +684,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tree_tc(TreeParams p) {
 #pragma unroll
                 for (int k = 0; k < 4; k++) big[k] = fmaxf(big[k], u[e + k]);
             float m_new = fmaxf(fmaxf(big[0], big[1]), fmaxf(big[2], big[3]));
-            m_new = fmaxf(m, fmaxf(m_new, meet(i, m_new)));
+            m_new = fmaxf(m, fmaf(fmaxf(m_new, meet(i, m_new)), factor, value_power));
             const bool fresh = (i * T::kKeys) % kFlushKeys == 0;   // O starts afresh with this tile
             const bool flush = fresh && i > 0;
             const bool move = !fresh && (m_new > m + kThreshold || (m == -INFINITY && m_new > -INFINITY));
@@ -747,7 +694,8 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tree_tc(TreeParams p) {
                 tc_fence_after();
             }
             if (flush) {
-                // O, relative to m, is added to what is in memory (or takes its place, where that is nothing beside it)
+                // O, relative to m, is added to what is in memory (or takes its place, where that is nothing beside it);
+                // a warp's 32 rows lie together there
                 const bool over = m_out == -INFINITY || m > m_out + 60.0f;
                 const float g = over ? 1.0f : exp2f(m - m_out);
 #pragma unroll 1
@@ -755,15 +703,15 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tree_tc(TreeParams p) {
                     unsigned v[32];
                     tmem_ld32(lane_at + kTmemO + 128 * half + 32 * j, v);
                     if (!live || *wait.abort) continue;
-                    float *const to = dst + dims_of(j);
 #pragma unroll
                     for (int e = 0; e < 32; e += 4) {
                         const float4 w = make_float4(__uint_as_float(v[e]) * g, __uint_as_float(v[e + 1]) * g,
                                                      __uint_as_float(v[e + 2]) * g, __uint_as_float(v[e + 3]) * g);
+                        float *const to = flushed + (size_t)(32 * half + 8 * j + e / 4) * (kRows * 4);
                         if (over)
-                            *reinterpret_cast<float4 *>(to + e) = w;
+                            *reinterpret_cast<float4 *>(to) = w;
                         else
-                            asm volatile("red.global.add.v4.f32 [%0], {%1, %2, %3, %4};" ::"l"(to + e), "f"(w.x), "f"(w.y),
+                            asm volatile("red.global.add.v4.f32 [%0], {%1, %2, %3, %4};" ::"l"(to), "f"(w.x), "f"(w.y),
                                          "f"(w.z), "f"(w.w)
                                          : "memory");
                     }
@@ -788,20 +736,16 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tree_tc(TreeParams p) {
                 l *= corr;
                 m = m_new;
             }
-            const float ref = (m == -INFINITY ? 0.0f : m) - kLift;
+            const float shift = value_power - ((m == -INFINITY ? 0.0f : m) - kLift);
             float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
             unsigned o[T::kHalf];
 #pragma unroll
-            for (int e = 0; e < T::kHalf; e += 4) {
-                const float4 g = vi[e / 4];
-                const float w0 = ex2(u[e] - ref), w1 = ex2(u[e + 1] - ref), w2 = ex2(u[e + 2] - ref), w3 = ex2(u[e + 3] - ref);
-                sum[0] = fmaf(w0, g.x, sum[0]);
-                sum[1] = fmaf(w1, g.y, sum[1]);
-                sum[2] = fmaf(w2, g.z, sum[2]);
-                sum[3] = fmaf(w3, g.w, sum[3]);
+            for (int e = 0; e < T::kHalf; e += 2) {
+                const float w0 = ex2(fmaf(u[e], factor, shift)), w1 = ex2(fmaf(u[e + 1], factor, shift));
+                sum[e & 2] += w0;
+                sum[(e & 2) + 1] += w1;
                 const int at = (e >> 4) * 16 + ((e & 15) >> 1);   // per 16 keys: eight words of hi, eight of lo
                 split_pair(w0, w1, o[at], o[at + 8]);
-                split_pair(w2, w3, o[at + 1], o[at + 9]);
             }
             if constexpr (T::kHalf == 32) {
                 tmem_st32(s_at, o);
@@ -811,7 +755,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tree_tc(TreeParams p) {
                 for (int e = 0; e < 16; e++) v[e] = __uint_as_float(o[e]);
                 tmem_st16(s_at, v);
             }
-            l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+            l = fmaf((sum[0] + sum[1]) + (sum[2] + sum[3]), value_inverse, l);
             tmem_wait_st();
             tc_fence_before();
             __syncwarp();
@@ -827,7 +771,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tree_tc(TreeParams p) {
             tc_fence_after();
             l += meet(n, l);
             // (O lacks the power that the values' are relative to)
-            const float inv = whole ? power(s_power0) / l : power(s_power0);
+            const float inv = whole ? power(power0) / l : power(power0);
             // part of the row may be in memory; where the last part outweighs that past all bounds, it is dropped
             const bool join = m_out != -INFINITY && m <= m_out + 60.0f;
             const float g = join ? exp2f(m_out - m) : 0.0f;
@@ -838,13 +782,15 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tree_tc(TreeParams p) {
                 float *const at = staged + r * kOutPitch + dims_of(j);
                 if (join && live) {
                     // (this thread's own stores and additions)
-#pragma unroll 1
-                    for (int e = 0; e < 32; e += 4) {
-                        const float4 old = __ldcg(reinterpret_cast<const float4 *>(dst + dims_of(j) + e));
-                        *reinterpret_cast<float4 *>(at + e) = make_float4(old.x * g, old.y * g, old.z * g, old.w * g);
-                    }
 #pragma unroll
-                    for (int e = 0; e < 32; e++) v[e] = __float_as_uint(__uint_as_float(v[e]) + at[e]);
+                    for (int e = 0; e < 32; e += 4) {
+                        const float4 old =
+                            __ldcg(reinterpret_cast<const float4 *>(flushed + (size_t)(32 * half + 8 * j + e / 4) * (kRows * 4)));
+                        v[e] = __float_as_uint(fmaf(old.x, g, __uint_as_float(v[e])));
+                        v[e + 1] = __float_as_uint(fmaf(old.y, g, __uint_as_float(v[e + 1])));
+                        v[e + 2] = __float_as_uint(fmaf(old.z, g, __uint_as_float(v[e + 2])));
+                        v[e + 3] = __float_as_uint(fmaf(old.w, g, __uint_as_float(v[e + 3])));
+                    }
                 }
 #pragma unroll
                 for (int e = 0; e < 32; e += 4)
