@@ -8,6 +8,8 @@
 // warp, and walks its run 32 cache rows at a time: the tile is dequantised once to f32 in shared memory for all of them
 // (scores: lane = cache row; values: lane = dims), so the cache is read once per 32 query rows and the products are plain
 // f32 FMAs, which bound it.
+#include <atomic>
+
 #include "q8_pack.cuh"
 #include "tree.cuh"
 
@@ -257,10 +259,17 @@ __global__ void __launch_bounds__(256) attn_tree_fold(TreeParams p) {
 template <int kB>
 int launch_scalar(cudaStream_t stream, const TreeParams &p) {
     constexpr int kD = 32 * kB;
-    constexpr size_t kSmem = (2 * (size_t)kKeys * (kD + 1) + (size_t)kRows * kD) * sizeof(float);
-    if (kSmem > 48 * 1024) {   // (per device; setting it again is cheap beside a launch)
+    constexpr size_t kNeed = (2 * (size_t)kKeys * (kD + 1) + (size_t)kRows * kD) * sizeof(float);
+    // Two CTAs to an SM and no more: launches start early, while others' CTAs are there, and then the few that have work came
+    // together on a few SMs (12 nodes of eight heads of 64 over 1,000 rows, calls in a row: 30.5 us).
+    constexpr size_t kSmem = kNeed > 80 * 1024 ? kNeed : 80 * 1024;
+    static std::atomic<bool> configured[64];
+    int dev = 0;
+    cudaGetDevice(&dev);
+    if (dev < 0 || dev >= 64 || !configured[dev].load()) {
         const cudaError_t e = cudaFuncSetAttribute(attn_tree_scalar<kB>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmem);
         if (e != cudaSuccess) return (int)e;
+        if (dev >= 0 && dev < 64) configured[dev].store(true);
     }
     return launch_pdl(attn_tree_scalar<kB>, dim3(p.grid), dim3(256), kSmem, stream, 1, p);
 }

@@ -20,15 +20,20 @@
 // A K row that is not finite is not a number in the planes, which reaches the rows that see it and no others; a V row that is
 // not finite is zero there, and the weights of those that see it are not a number (a hidden key's weight is 0).
 //
-// Where the time goes (a quantised tile of 64 rows): tensor pipe 2 x 1,536 cycles; shared memory 7.1 KB a row: the raw
-// bytes in and out (1.1), the planes (2), K and the low part of Q into the pipe (2.5), V (1.5), 55 cycles a row at 128
-// bytes a cycle. So the pipe and shared memory are about balanced, and Q's high part and W come from TMEM for that reason:
-// Q hi takes 128 of the 512 columns, O 256, two S tiles 128.
+// Where the time goes (a quantised tile of 64 rows): the MMAs 3,330 cycles (48 of N = 64, 32 cycles with A from TMEM and 48
+// with A from shared memory, and 24 of N = 128, 64 cycles); shared memory as much: the raw bytes in and out (1.1 KB a row),
+// the planes (2), K and the low part of Q into the pipe (2.5), V (1.5), 55 cycles a row. So Q's high part and W come from
+// TMEM: Q hi takes 128 of the 512 columns, O 256, two S tiles 128. A tile takes 5,400 to 6,000 cycles, 64 nodes of eight
+// heads over 100,000 rows 480 us (of a run under the power cap 530): both products and the planes share the issue slots of
+// 20 warps. One warp group more for the planes (24 warps) changed nothing, nor did a third stage of V.
+// Short calls are bound by what comes before the first tile: the launch, the tree, Q's planes, one trip to memory after
+// another and the code's own lines (the loops are loops for that reason).
 //
 // Sums: the tensor cores cut their f32 accumulators off instead of rounding them, 3.5e-9 relative per key of an unbroken
 // chain, so every kFlushKeys keys O leaves TMEM for the run's partial in memory (added there, in f32).
 //
-// Warps 0-7 softmax and epilogue, 8-11 planes of K, 12-15 of V, 16 copies, 17 the factors of V's rows, 19 MMAs
+// Warps 0-7 softmax and epilogue, 8-11 planes of K, 12-15 of V, 16 copies, 17 the largest of a tile's V
+// rows and their factors, 18 those of K, 19 MMAs
 // (the whole warp runs that loop and one elected lane issues: from a branch of a single lane every descriptor went through a
 // move to the uniform registers, 46 cycles an MMA of N = 64 and 83 beside the other warps, against 32; the fourth scheduler
 // has the fewest other warps). Waits are bounded: one that runs out sets the device
@@ -217,7 +222,7 @@ __device__ __forceinline__ void block_planes(const unsigned *w, unsigned take, _
     }
 }
 
-// grid tree_grid(.., 128 rows, the device's SMs), 18 warps.
+// grid tree_grid(.., 128 rows, the device's SMs), 20 warps.
 template <int kType>
 __global__ void __launch_bounds__(kThreads, 1) attn_tree_tc(TreeParams p) {
     using T = Shape<kType>;
@@ -531,7 +536,6 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tree_tc(TreeParams p) {
         auto free_raw = [&](unsigned u) {
             if (lane == 0) mbar_arrive(raw_empty + 8 * (u % T::kRawSlots));
         };
-        if (!is_v && n > 0) named_sync(7, 12 * 32);   // Q hi has left K's stages
         unsigned c = 0;                               // stages written
 #pragma unroll 1
         for (int t = 0; t < n; t++) {
@@ -574,6 +578,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tree_tc(TreeParams p) {
                     block_planes<kType>(w, h ? 0x7654 : 0x5432, __float2half2_rn(by == 0.0f ? 0.0f : scale * by), hi, lo);
                 }
                 if (bad && !is_v) hi[0] = 0x7fff7fff;   // one value is enough: the row's scores are not a number
+                if (!is_v && c == 0 && j == 0) named_sync(7, 12 * 32);   // Q hi has left K's stages
                 if (is_v || j == 0) wait((is_v ? v_empty : k_empty) + 8 * (c % kStages), ((c / kStages) & 1) ^ 1, 55);
                 const int b = kType == 0 ? blk : pair;
                 unsigned char *const dst = is_v ? smem + kOffV + (c % kStages) * kVStage + row * 128 + (b >> 1) * T::kVChunkBytes
@@ -738,22 +743,20 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tree_tc(TreeParams p) {
             }
             const float shift = value_power - ((m == -INFINITY ? 0.0f : m) - kLift);
             float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-            unsigned o[T::kHalf];
 #pragma unroll
-            for (int e = 0; e < T::kHalf; e += 2) {
-                const float w0 = ex2(fmaf(u[e], factor, shift)), w1 = ex2(fmaf(u[e + 1], factor, shift));
-                sum[e & 2] += w0;
-                sum[(e & 2) + 1] += w1;
-                const int at = (e >> 4) * 16 + ((e & 15) >> 1);   // per 16 keys: eight words of hi, eight of lo
-                split_pair(w0, w1, o[at], o[at + 8]);
-            }
-            if constexpr (T::kHalf == 32) {
-                tmem_st32(s_at, o);
-            } else {
-                float v[16];
+            for (int e0 = 0; e0 < T::kHalf; e0 += 16) {   // per 16 keys: eight words of hi, eight of lo
+                float o[16];
 #pragma unroll
-                for (int e = 0; e < 16; e++) v[e] = __uint_as_float(o[e]);
-                tmem_st16(s_at, v);
+                for (int e = 0; e < 16; e += 2) {
+                    const float w0 = ex2(fmaf(u[e0 + e], factor, shift)), w1 = ex2(fmaf(u[e0 + e + 1], factor, shift));
+                    sum[e & 2] += w0;
+                    sum[(e & 2) + 1] += w1;
+                    unsigned hi, lo;
+                    split_pair(w0, w1, hi, lo);
+                    o[e / 2] = __uint_as_float(hi);
+                    o[8 + e / 2] = __uint_as_float(lo);
+                }
+                tmem_st16(s_at + e0, o);
             }
             l = fmaf((sum[0] + sum[1]) + (sum[2] + sum[3]), value_inverse, l);
             tmem_wait_st();

@@ -22,18 +22,20 @@ __global__ void __launch_bounds__(kThreads) kv_path_keep(const __grid_constant__
     griddep_wait();
     const int tid = threadIdx.x, slot = blockIdx.y;
     const int which = blockIdx.x / p.n_kv, head = blockIdx.x - which * p.n_kv;
+    // (the path is fetched whole, beside its length: one trip to memory)
+    static_assert(kThreads >= kTreeNodes, "a thread per node");
+    int node = -1, before = -1;
+    if (tid < p.nodes) {
+        const int *const at = p.path + (size_t)slot * p.nodes + tid;
+        node = __ldcg(at);
+        if (tid > 0) before = __ldcg(at - 1);
+    }
     const TreeSlot t = tree_slot(p.pos, slot, p.stride, p.nodes);
     const int count = __ldcg(p.count + slot);
-    if (count < 0 || count > t.live) {
-        if (tid == 0) atomicCAS(p.status, 0, kTreeBadPath);
-        return;
-    }
-    bool bad = false;
-    for (int i = tid; i < count; i += kThreads) {
-        const int *const at = p.path + (size_t)slot * p.nodes + i;
-        const int node = __ldcg(at), before = i > 0 ? __ldcg(at - 1) : -1;
+    bool bad = count < 0 || count > t.live;
+    if (tid < count) {
         bad = bad || node <= before || node < 0 || node >= t.live;
-        s_path[i] = node;
+        s_path[tid] = node;
     }
     if (__syncthreads_or(bad)) {   // the slot's rows stay as they are
         if (tid == 0) atomicCAS(p.status, 0, kTreeBadPath);

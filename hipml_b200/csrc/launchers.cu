@@ -918,6 +918,20 @@ static int check_slot_bytes(int kv_dtype, int n_kv, int head_dim, int stride, in
     return 0;
 }
 
+// The device status word, looked up once per device (an engine makes these calls once per layer).
+static int *status_of_device() {
+    static std::atomic<int *> found[64];
+    int dev = 0;
+    cudaGetDevice(&dev);
+    if (dev < 0 || dev >= 64) return device_status_word();
+    int *p = found[dev].load();
+    if (!p) {
+        p = device_status_word();
+        found[dev].store(p);
+    }
+    return p;
+}
+
 // CTAs of the two kernels of tree attention: one or two to an SM.
 static int tree_grid_of(bool tensor_core, int n_heads, int n_kv, int nodes, int slots) {
     return tensor_core ? tree_grid(n_heads, n_kv, nodes, slots, kTreeTcRows, device_sms())
@@ -953,7 +967,7 @@ int hipml_attn_tree(hipml_stream_t stream, int kv_dtype, const int *pos, const i
     if ((reinterpret_cast<size_t>(workspace) & 15) != 0)
         return fail(HIPML_ERR_WORKSPACE, "tree attention workspace must be 16-byte aligned");
     TreeParams p;
-    p.status = device_status_word();
+    p.status = status_of_device();
     if (!p.status) return launch_status();
     p.pos = pos;
     p.parents = parents;
@@ -993,7 +1007,7 @@ int hipml_tree_verify(hipml_stream_t stream, const int *pos, const int *parents,
         return fail(HIPML_ERR_INVALID_ARGUMENT, "rows of %lld probabilities for %d tokens", row_stride, vocab);
     if (!pos || !parents || !tokens || !target || !uniform || !path || !count || !next)
         return fail(HIPML_ERR_INVALID_ARGUMENT, "tree verification: a tensor is missing");
-    VerifyParams p = {pos, parents, tokens, target, draft, uniform, path, count, next, device_status_word(),
+    VerifyParams p = {pos, parents, tokens, target, draft, uniform, path, count, next, status_of_device(),
                       nodes, slots, vocab, row_stride};
     if (!p.status) return launch_status();
     return launch_tree_verify(as_stream(stream), p);
@@ -1021,7 +1035,7 @@ int hipml_kv_path_keep(hipml_stream_t stream, int kv_dtype, const int *pos, cons
     p.pos = pos;
     p.path = path;
     p.count = count;
-    p.status = device_status_word();
+    p.status = status_of_device();
     if (!p.status) return launch_status();
     p.n_kv = n_kv;
     p.stride = stride;

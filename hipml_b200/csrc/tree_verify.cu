@@ -8,12 +8,15 @@
 // Accepted tokens and the drawn one are distributed as the target's own (the drafter's errors cost speed only).
 // No counterpart in the reference, which compares greedy tokens on the host (crates/hipml-model/src/gpu/spec.rs).
 //
-// A slot is one cluster of CTAs; each has a part of the vocabulary. What the walk asks of single tokens, r(x) and q(x) of
-// every node, is fetched by all nodes at once in the beginning (one trip to memory instead of one per level); a rejected
-// child costs one pass over the target and the draft row, all CTAs together, and the pass of the last rejection leaves the
-// sums by which the next token is found (no rejection: one pass over the target row). Differences, sums and comparisons are
-// in 64 bits: over 150,000 probabilities a 32-bit running sum moves some thousandth of the drawn tokens by one place. r of
-// the second and later rejections is computed from the rows again, so nothing is kept per probability.
+// A slot is one cluster of CTAs; each has a part of the vocabulary, each warp a run of that. What the walk asks of single
+// tokens, r(x) and q(x) of every node, is fetched by all nodes at once in the beginning (one trip to memory instead of one
+// per level). A rejected child costs one pass over the target and the draft row, all CTAs together; without draft rows only
+// the first one of a node does, the others take their token's probability off the sum. The sums of the last pass are those by
+// which the next token is found (another one where it was not over all that was rejected). Differences, sums and comparisons
+// are in 64 bits: over 150,000 probabilities a 32-bit running sum moves some thousandth of the drawn tokens by one place. r
+// after the second and later rejections is computed from the rows again, so nothing is kept per probability.
+#include <atomic>
+
 #include "sm100_ptx.cuh"
 #include "tree.cuh"
 
@@ -23,10 +26,8 @@ namespace {
 
 using namespace ptx;
 
-constexpr int kCtas = 8, kThreads = 512, kWarps = kThreads / 32;
-constexpr int kPiece = kThreads * 4;      // probabilities that a CTA takes at once
-constexpr int kSegment = 128;             // of a warp: what the sums are kept of
-constexpr int kSegments = kVerifyVocab / kCtas / kSegment;
+constexpr int kThreads = 512, kWarps = kThreads / 32;
+constexpr int kAtOnce = 8;                // a lane's probabilities that are on their way together
 
 // The rejections since a node was kept, by which what is left of its target row is computed.
 struct Left {
@@ -44,43 +45,60 @@ __device__ __forceinline__ double warp_sum_f64(double v) {
     return v;
 }
 
-__global__ void __launch_bounds__(kThreads) __cluster_dims__(kCtas, 1, 1) tree_verify(VerifyParams p) {
+// The sum of non-negative f32 values with their rounding errors, to about 2^-46 of it.
+struct LongSum {
+    float hi = 0.0f, lo = 0.0f;
+    __device__ __forceinline__ void add(float x, float error) {
+        const float s = hi + x, b = s - hi;
+        lo += ((hi - (s - b)) + (x - b)) + error;
+        hi = s;
+    }
+};
+
+// grid slots * kCtas, clusters of kCtas.
+template <int kCtas>
+__global__ void __launch_bounds__(kThreads) tree_verify(VerifyParams p) {
     __shared__ int s_parent[kTreeNodes], s_token[kTreeNodes];
     __shared__ float s_u[kTreeNodes], s_p[kTreeNodes], s_q[kTreeNodes];
     __shared__ Left s_left;
-    __shared__ double s_segment[kSegments];   // of this CTA's part
     __shared__ double s_sum[2];               // this CTA's part of a pass, read by the others (the passes take turns)
-    __shared__ double s_all[kCtas];
-    __shared__ double s_warp[kWarps];
+    __shared__ double s_all[kCtas];           // the sums of the parts
+    __shared__ double s_warp[kWarps];         // of this part, by warp
+    __shared__ double s_segment[kWarps];
+    static_assert(kThreads >= kTreeNodes, "a thread per node");
     griddep_launch();
     griddep_wait();
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int rank = (int)cluster_rank(), slot = blockIdx.x / kCtas;
+    const size_t first = (size_t)slot * p.nodes;
+    // (a thread per node, dead ones too: the slot's length comes with the same trip to memory)
+    int up = -1, x_of = 0;
+    if (tid < p.nodes) {
+        up = tid == 0 ? -1 : __ldcg(p.parents + first + tid);
+        x_of = tid == 0 ? 0 : __ldcg(p.tokens + first + tid);
+        s_u[tid] = __ldcg(p.uniform + first + tid);
+    }
     const TreeSlot t = tree_slot(p.pos, slot, 0x7fffffff, p.nodes);
     if (t.live == 0) return;   // (the whole cluster) nothing is written
-    const size_t first = (size_t)slot * p.nodes;
-    bool bad = false;
-    for (int i = tid; i < t.live; i += kThreads) {
-        int up = i == 0 ? -1 : p.parents[first + i], x = i == 0 ? 0 : p.tokens[first + i];
-        if (up >= i || up < -1) bad = true, up = -1;
-        if (x < 0 || x >= p.vocab) bad = true, up = -1;   // (is not reached)
-        s_parent[i] = up;
-        s_token[i] = x;
-        s_u[i] = p.uniform[first + i];
+    if (tid < t.live) {
+        if (up >= tid || up < -1 || x_of < 0 || x_of >= p.vocab) {
+            if (rank == 0) atomicCAS(p.status, 0, kTreeBadTree);
+            up = -1;           // (is not reached)
+            x_of = 0;
+        }
+        s_parent[tid] = up;
+        s_token[tid] = x_of;
         if (up >= 0) {
-            const long long at = (long long)(first + up) * p.row_stride + x;
-            s_p[i] = p.target[at];
-            s_q[i] = p.draft ? p.draft[at] : 1.0f;
+            const long long at = (long long)(first + up) * p.row_stride + x_of;
+            s_p[tid] = __ldg(p.target + at);
+            s_q[tid] = p.draft ? __ldg(p.draft + at) : 1.0f;
         }
     }
-    if (bad && rank == 0) atomicCAS(p.status, 0, kTreeBadTree);
     __syncthreads();
 
-    // this CTA's part of the vocabulary, in whole pieces of four
-    const int quads = (p.vocab + 3) / 4, part = (quads + kCtas - 1) / kCtas * 4;
+    // this CTA's part of the vocabulary and the warps' runs of it (rows may lie anywhere: a lane loads single values)
+    const int run = (p.vocab + kCtas * kWarps - 1) / (kCtas * kWarps), part = run * kWarps;
     const int v0 = min(rank * part, p.vocab), v1 = min(v0 + part, p.vocab);
-    const bool wide = ((reinterpret_cast<size_t>(p.target) | reinterpret_cast<size_t>(p.draft)) & 15) == 0 &&
-                      (p.row_stride & 3) == 0;
     int here = 0;   // the node that was kept last
 
     // what is left of p.target's row `here` at x, before the division by the last sum; `tried` rejections
@@ -93,43 +111,75 @@ __global__ void __launch_bounds__(kThreads) __cluster_dims__(kCtas, 1, 1) tree_v
         }
         return r;
     };
-    // four probabilities from x on
-    auto load4 = [&](const float *row, int x, float (&v)[4]) {
-        if (wide && x + 4 <= v1) {
-            const float4 w = __ldg(reinterpret_cast<const float4 *>(row + x));
-            v[0] = w.x, v[1] = w.y, v[2] = w.z, v[3] = w.w;
-        } else {
-#pragma unroll
-            for (int e = 0; e < 4; e++) v[e] = x + e < v1 ? __ldg(row + x + e) : 0.0f;
-        }
-    };
-    // One pass over the row: the sums of this CTA's segments, and the sum of all (in the order of the CTAs, everywhere the
-    // same bits).
+    // One pass over the row: the sums of the warps' runs, and the sum of all (everywhere the same bits). `known`: how many of
+    // the rejections the runs' sums have in them already (-1: they are of another row); without draft rows only runs that
+    // have lost a token since are summed again.
     int passes = 0;
-    auto pass = [&](int tried) {
+    auto pass = [&](int tried, int known) {
         const float *const target = p.target + (long long)(first + here) * p.row_stride;
-        const float *const draft = p.draft ? p.draft + (long long)(first + here) * p.row_stride : nullptr;
-        double mine = 0.0;
-        for (int x0 = v0, n = 0; x0 < v1; x0 += kPiece, n++) {
-            const int x = x0 + 4 * tid;
-            float a[4] = {0.0f, 0.0f, 0.0f, 0.0f}, b[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-            if (x < v1) {
-                load4(target, x, a);
-                if (draft && tried > 0) load4(draft, x, b);
-            }
-            double sum = 0.0;
+        const float *const draft = p.draft && tried > 0 ? p.draft + (long long)(first + here) * p.row_stride : nullptr;
+        const int w0 = min(v0 + warp * run, v1), w1 = min(w0 + run, v1);
+        // Most often what is left is p or max(p - q, 0): in f32 with the rounding error beside it, which is as exact here and
+        // an eighth of the instructions in 64 bits. (The loops are loops: this code runs once or twice a launch, and its
+        // lines come from beyond the instruction cache: unrolled in 64 bits 8 nodes of 151,936 took 30 us, so 12. Sixteen
+        // values at once take 80 registers, which leaves an SM one CTA: 32 slots of 8 nodes 62 us, with eight 32.)
+        bool again = p.draft || known < 0;
+        if (!again)
+            for (int j = known; j < tried; j++) again = again || (s_left.token[j] >= w0 && s_left.token[j] < w1);
+        double sum = 0.0;
+        if (!again) {
+            sum = lane == 0 ? s_warp[warp] : 0.0;
+        } else if (!p.draft || tried <= 1) {
+            LongSum s;
+#pragma unroll 1
+            for (int x0 = w0 + lane; x0 < w1; x0 += 32 * kAtOnce) {
+                float a[kAtOnce], b[kAtOnce];
 #pragma unroll
-            for (int e = 0; e < 4; e++) sum += left_of(probability(a[e]), probability(b[e]), x + e, tried);
-            sum = warp_sum_f64(sum);
-            if (lane == 0) s_segment[n * kWarps + warp] = sum;
-            mine += sum;
+                for (int k = 0; k < kAtOnce; k++) {
+                    const int x = x0 + 32 * k;
+                    a[k] = x < w1 ? __ldg(target + x) : 0.0f;
+                    b[k] = draft && x < w1 ? __ldg(draft + x) : 0.0f;
+                }
+                if (!p.draft) {   // what was rejected is no longer there
+#pragma unroll 1
+                    for (int j = 0; j < tried; j++) {
+                        const int gone = s_left.token[j] - x0;
+                        if (gone < -lane || gone >= 32 * kAtOnce - lane) continue;   // (the same in every lane)
+#pragma unroll
+                        for (int k = 0; k < kAtOnce; k++)
+                            if (gone == 32 * k) a[k] = 0.0f;
+                    }
+                }
+#pragma unroll
+                for (int k = 0; k < kAtOnce; k++) {
+                    const float u = a[k] > 0.0f && a[k] < INFINITY ? a[k] : 0.0f;   // as probability()
+                    const float v = b[k] > 0.0f && b[k] < INFINITY ? b[k] : 0.0f;
+                    const float d = u - v, e = d - u;
+                    if (d > 0.0f) s.add(d, (u - (d - e)) - (v + e));
+                }
+            }
+            sum = (double)s.hi + (double)s.lo;
+        } else {
+            constexpr int kFew = 4;
+#pragma unroll 1
+            for (int x0 = w0 + lane; x0 < w1; x0 += 32 * kFew) {
+                float a[kFew], b[kFew];
+#pragma unroll
+                for (int k = 0; k < kFew; k++) {
+                    const int x = x0 + 32 * k;
+                    a[k] = x < w1 ? __ldg(target + x) : 0.0f;
+                    b[k] = x < w1 ? __ldg(draft + x) : 0.0f;
+                }
+#pragma unroll
+                for (int k = 0; k < kFew; k++) sum += left_of(probability(a[k]), probability(b[k]), x0 + 32 * k, tried);
+            }
         }
-        if (lane == 0) s_warp[warp] = mine;
+        sum = warp_sum_f64(sum);
+        if (lane == 0) s_warp[warp] = sum;
         __syncthreads();
-        if (tid == 0) {
-            double all = 0.0;
-            for (int w = 0; w < kWarps; w++) all += s_warp[w];
-            s_sum[passes & 1] = all;
+        if (warp == 0) {
+            const double all = warp_sum_f64(lane < kWarps ? s_warp[lane] : 0.0);
+            if (lane == 0) s_sum[passes & 1] = all;
         }
         cluster_sync_all();
         if (tid < kCtas) {
@@ -140,16 +190,16 @@ __global__ void __launch_bounds__(kThreads) __cluster_dims__(kCtas, 1, 1) tree_v
         }
         __syncthreads();
         passes++;
-        double all = 0.0;
-        for (int c = 0; c < kCtas; c++) all += s_all[c];
-        return all;
+        return warp_sum_f64(lane < kCtas ? s_all[lane] : 0.0);
     };
 
     // The walk, the same in every thread. An accepted child lies behind its parent and its siblings are tried in order, so
     // one run over the nodes meets them all.
     int count = 1, tried = 0;
-    bool summed = false;      // the last pass was over what is left now
+    bool counted = false;     // `whole` is the sum of what is left now
+    int known = -1;           // rejections that the sums of the last pass have in them
     double whole = 1.0;       // what r is divided by
+    double least = 0.0;       // down to what `whole` may be taken less without another pass
     if (rank == 0 && tid == 0) p.path[first] = 0;
     for (int i = 1; i < t.live; i++) {
         if (s_parent[i] != here) continue;
@@ -162,7 +212,8 @@ __global__ void __launch_bounds__(kThreads) __cluster_dims__(kCtas, 1, 1) tree_v
             count++;
             tried = 0;
             whole = 1.0;
-            summed = false;
+            counted = false;
+            known = -1;
             continue;
         }
         __syncthreads();
@@ -171,16 +222,21 @@ __global__ void __launch_bounds__(kThreads) __cluster_dims__(kCtas, 1, 1) tree_v
             if (tried > 0) s_left.inverse[tried - 1] = 1.0 / whole;
         }
         __syncthreads();
-        const double sum = pass(tried + 1);
+        double sum;
+        if (!p.draft && counted && whole - r >= least) {
+            sum = whole - r;   // (r is 0 if the token has left before)
+        } else {
+            sum = pass(tried + 1, known);
+            known = sum > 0.0 ? tried + 1 : -1;
+            least = sum * 0x1p-10;   // (the rounding of what is taken away stays 2^-43 of what is left)
+        }
         if (sum > 0.0) {
             tried++;
             whole = sum;
-            summed = true;
-        } else {
-            summed = false;   // (the segments' sums are of nothing)
+            counted = true;
         }
     }
-    if (!summed) whole = pass(tried);
+    if (known != tried) whole = pass(tried, known);
     if (rank == 0) {
         for (int i = count + tid; i < p.nodes; i += kThreads) p.path[first + i] = -1;
         if (tid == 0) p.count[slot] = count;
@@ -190,88 +246,77 @@ __global__ void __launch_bounds__(kThreads) __cluster_dims__(kCtas, 1, 1) tree_v
     if (!(whole > 0.0)) {
         if (rank == 0 && tid == 0) p.next[slot] = -1;
     } else {
-        double before = 0.0;
-        int owner = -1, last = 0;   // last: the part that ends the mass, where rounding leaves no running sum above the bar
-        double upto = 0.0, before_last = 0.0;
-        for (int c = 0; c < kCtas; c++) {
-            if (s_all[c] > 0.0) {
-                last = c;
-                before_last = upto;
-            }
-            if (owner < 0 && upto + s_all[c] > bar && s_all[c] > 0.0) {
-                owner = c;
-                before = upto;
-            }
-            upto += s_all[c];
-        }
-        const bool end = owner < 0;   // the last token that has mass
-        if (end) {
-            owner = last;
-            before = before_last;
-        }
-        if (rank == owner && warp == 0) {
-            const int segments = (v1 - v0 + kSegment - 1) / kSegment;
-            int at = -1, at_last = 0;
-            double start = before, start_last = before;
-            for (int s0 = 0; s0 < segments; s0 += 32) {
-                const double mine = s0 + lane < segments ? s_segment[s0 + lane] : 0.0;
-                double incl = mine;
-#pragma unroll
-                for (int o = 1; o < 32; o <<= 1) {
-                    const double w = __shfl_up_sync(0xffffffffu, incl, o);
-                    if (lane >= o) incl += w;
-                }
-                const unsigned some = __ballot_sync(0xffffffffu, mine > 0.0);
-                const unsigned past = end ? 0 : __ballot_sync(0xffffffffu, mine > 0.0 && before + incl > bar);
-                if (past && at < 0) {
-                    const int l = __ffs(past) - 1;
-                    at = s0 + l;
-                    start = before + __shfl_sync(0xffffffffu, incl - mine, l);
-                }
-                if (some) {
-                    const int l = 31 - __clz(some);
-                    at_last = s0 + l;
-                    start_last = before + __shfl_sync(0xffffffffu, incl - mine, l);
-                }
-                before += __shfl_sync(0xffffffffu, incl, 31);
-            }
-            if (at < 0) {
-                at = at_last;
-                start = start_last;
-            }
-            const float *const target = p.target + (long long)(first + here) * p.row_stride;
-            const float *const draft = p.draft ? p.draft + (long long)(first + here) * p.row_stride : nullptr;
-            const int x = v0 + at * kSegment + 4 * lane;
-            float a[4] = {0.0f, 0.0f, 0.0f, 0.0f}, b[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-            if (x < v1) {
-                load4(target, x, a);
-                if (draft && tried > 0) load4(draft, x, b);
-            }
-            double w[4], incl = 0.0;
-#pragma unroll
-            for (int e = 0; e < 4; e++) {
-                w[e] = left_of(probability(a[e]), probability(b[e]), x + e, tried);
-                incl += w[e];
-            }
-            const double mine = incl;
-#pragma unroll
+        // Of up to 32 sums (a lane has one) the first within which the running sum, from `before` on, passes the bar, or the
+        // last that is not 0 where none does; `before` becomes the running sum in front of it.
+        auto choose = [&](double mine, double &before, bool &past) {
+            double incl = mine;
+#pragma unroll 1
             for (int o = 1; o < 32; o <<= 1) {
                 const double v = __shfl_up_sync(0xffffffffu, incl, o);
                 if (lane >= o) incl += v;
             }
-            double c = start + incl - mine;
+            const unsigned over = __ballot_sync(0xffffffffu, mine > 0.0 && before + incl > bar);
+            const unsigned some = __ballot_sync(0xffffffffu, mine > 0.0);
+            const int at = over ? __ffs(over) - 1 : 31 - __clz(some);
+            before += __shfl_sync(0xffffffffu, incl - mine, at);
+            past = over != 0;
+            return at;
+        };
+        double start = 0.0;
+        bool past;
+        const int owner = choose(lane < kCtas ? s_all[lane] : 0.0, start, past);
+        if (rank == owner) {
+            // the warp's run in the part; every warp of the CTA finds it alike
+            const int at = choose(lane < kWarps ? s_warp[lane] : 0.0, start, past);
+            const float *const target = p.target + (long long)(first + here) * p.row_stride;
+            const float *const draft = p.draft && tried > 0 ? p.draft + (long long)(first + here) * p.row_stride : nullptr;
+            const int w0 = min(v0 + at * run, v1), w1 = min(w0 + run, v1);
             int found = 0x7fffffff, ends = -1;
-#pragma unroll
-            for (int e = 0; e < 4; e++) {
-                c += w[e];
-                if (w[e] > 0.0) {
-                    ends = x + e;
-                    if (c > bar && found == 0x7fffffff) found = x + e;
+            // its segments of 32, one to a warp and round: their sums, then the one in which the running sum passes the bar
+#pragma unroll 1
+            for (int x0 = w0; x0 < w1; x0 += 32 * kWarps) {
+                const int x = x0 + 32 * warp + lane;
+                double w = 0.0;
+                if (x < w1) w = left_of(probability(__ldg(target + x)), draft ? probability(__ldg(draft + x)) : 0.0, x, tried);
+                double incl = w;
+#pragma unroll 1
+                for (int o = 1; o < 32; o <<= 1) {
+                    const double v = __shfl_up_sync(0xffffffffu, incl, o);
+                    if (lane >= o) incl += v;
+                }
+                if (lane == 31) s_segment[warp] = incl;
+                __syncthreads();
+                double sums = lane < kWarps ? s_segment[lane] : 0.0;
+#pragma unroll 1
+                for (int o = 1; o < kWarps; o <<= 1) {
+                    const double v = __shfl_up_sync(0xffffffffu, sums, o);
+                    if (lane >= o) sums += v;
+                }
+                double c = start + incl;
+                const double ahead = __shfl_sync(0xffffffffu, sums, warp > 0 ? warp - 1 : 0);
+                if (warp > 0) c += ahead;
+                start += __shfl_sync(0xffffffffu, sums, kWarps - 1);
+                __syncthreads();
+                if (w > 0.0) {
+                    ends = x;
+                    if (c > bar && found == 0x7fffffff) found = x;
                 }
             }
             found = __reduce_min_sync(0xffffffffu, found);
             ends = __reduce_max_sync(0xffffffffu, ends);
-            if (lane == 0) p.next[slot] = !end && found != 0x7fffffff ? found : ends;
+            // (s_parent and s_token have been read for the last time)
+            if (lane == 0) {
+                s_parent[warp] = found;
+                s_token[warp] = ends;
+            }
+            __syncthreads();
+            if (tid == 0) {
+                for (int k = 0; k < kWarps; k++) {
+                    found = min(found, s_parent[k]);
+                    ends = max(ends, s_token[k]);
+                }
+                p.next[slot] = found != 0x7fffffff ? found : ends;
+            }
         }
     }
     cluster_sync_all();   // no CTA leaves while another may still read its sum
@@ -279,8 +324,52 @@ __global__ void __launch_bounds__(kThreads) __cluster_dims__(kCtas, 1, 1) tree_v
 
 }  // namespace
 
+namespace {
+
+// Whether the current device runs a cluster of sixteen CTAs of the kernel.
+bool sixteen_together() {
+    if (cudaFuncSetAttribute(tree_verify<16>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess) {
+        cudaGetLastError();
+        return false;
+    }
+    cudaLaunchAttribute size = {};
+    size.id = cudaLaunchAttributeClusterDimension;
+    size.val.clusterDim.x = 16;
+    size.val.clusterDim.y = size.val.clusterDim.z = 1;
+    cudaLaunchConfig_t config = {};
+    config.gridDim = dim3(16);
+    config.blockDim = dim3(kThreads);
+    config.attrs = &size;
+    config.numAttrs = 1;
+    int clusters = 0;
+    if (cudaOccupancyMaxActiveClusters(&clusters, tree_verify<16>, &config) != cudaSuccess) {
+        cudaGetLastError();
+        return false;
+    }
+    return clusters > 0;
+}
+
+}  // namespace
+
+// Few slots take clusters of sixteen, which is more than every device must have and is asked for once; many fill it by eights.
+// What bounds it is latency, not memory: a trip for the tree, one for what the walk asks, one pass, the exchange of its sums
+// and the segment of the drawn token follow one another. 8 nodes of 151,936 take 11.6 us (16 slots' rows would pass in 3),
+// 8 slots of 16 nodes of 50,257 with draft rows 17.5 (several rejections in a row, a pass each), 32 slots of 8 nodes of
+// 151,936 without draft rows 32, of which the bytes take 3: the slots are not all there at once.
 int launch_tree_verify(cudaStream_t stream, const VerifyParams &p) {
-    return launch_pdl(tree_verify, dim3(p.slots * kCtas), dim3(kThreads), 0, stream, 1, p);
+    if (p.slots * 16 <= device_sms()) {
+        static std::atomic<int> sixteen[64];   // 0: not asked yet, 1: works, 2: does not
+        int dev = 0;
+        cudaGetDevice(&dev);
+        const bool known = dev >= 0 && dev < 64;
+        int works = known ? sixteen[dev].load() : 0;
+        if (works == 0) {
+            works = sixteen_together() ? 1 : 2;
+            if (known) sixteen[dev].store(works);
+        }
+        if (works == 1) return launch_pdl(tree_verify<16>, dim3(p.slots * 16), dim3(kThreads), 0, stream, 16, p);
+    }
+    return launch_pdl(tree_verify<8>, dim3(p.slots * 8), dim3(kThreads), 0, stream, 8, p);
 }
 
 }  // namespace hipml

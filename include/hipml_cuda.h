@@ -463,7 +463,7 @@ int hipml_attn_chunk_staged_gated(hipml_stream_t stream, const float *q, float *
  * nodes), the step words of the other entries: the drafted rows lie behind the prefix, node i's in
  * cache row base + i (append them with hipml_kv_encode_bulk, hipml_kv_append_cols_f32 or
  * hipml_attn_front_append_q8). parents is device i32 [slots][nodes]: the parent of node i, an
- * earlier node (< i), or -1. Nothing of a node past a slot's live ones is read or written, whatever
+ * earlier node (< i), or -1. Nothing of a node past a slot's live ones is used or written, whatever
  * the buffers hold there; lengths past the cache count as the cache. kv_dtype, caches and stride
  * are those of hipml_attn_chunk (0 f32 [stride][n_kv*head_dim], 1 q8_0, 2 q4_0 head-major), slot s
  * begins at byte s*kv_slot_bytes (any value where slots is 1). 1..65535 slots. A parent that is no
