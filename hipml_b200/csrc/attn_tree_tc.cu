@@ -62,7 +62,7 @@ constexpr int kRawBytes = 3 * 64 * 272;
 constexpr int kFlushKeys = 512;
 constexpr unsigned kSpinLimit = 1u << 22;
 constexpr float kThreshold = 8.0f;               // log2: the reference moves when a weight would exceed 2^8 times it,
-constexpr float kLift = 7.0f;                    // and weights are kept 2^7 times larger: below 2^15, f16's smallest 2^-24
+constexpr float kLift = 7.0f;                    // and weights are kept 2^7 times larger: up to 2^15.5, f16's smallest 2^-24
 constexpr int kLeastPower = -100, kMostPower = 100;   // of a tile; smaller values count as 0 (as do zeros)
 
 template <int kType>   // 0 f32, 1 q8_0, 2 q4_0
@@ -76,7 +76,7 @@ struct Shape {
     static constexpr int kVKeys = kKeys / 2;
     static constexpr int kVChunkBytes = kVKeys * 128;
     static constexpr int kVPlaneBytes = kChunks * kVChunkBytes;
-    static_assert(2 * kPlaneBytes == kKStage && 2 * kVPlaneBytes == kVStage, "a stage is two planes");
+    static_assert(kParts <= kStages && 2 * kPlaneBytes == kKStage && 2 * kVPlaneBytes == kVStage, "a stage is two planes");
     // the raw ring has half tiles (f32 rows padded apart so that eight rows' 16-byte words fall into different banks)
     static constexpr int kRowPitch = kType == 0 ? 1040 : (kType == 1 ? 272 : 144);
     static constexpr int kRawRows = kKeys / 2;
@@ -428,16 +428,18 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tree_tc(TreeParams p) {
                 tc_fence_after();
             };
             auto qk = [&](int i) {
-                const unsigned d = tmem + kTmemS + 64 * (i & 1);
+                const unsigned d = tmem + kTmemS + 64 * (i & 1), planes = desc_lo_sw128(smem_u32(smem + kOffK));
+                // The small terms of the whole row first, the large ones last: each MMA cuts the sum off, relative to what it
+                // has come to. (By parts, each with its small and large terms, the error of S was twice as large.)
 #pragma unroll 1
-                for (int h = 0; h < T::kParts; h++, kc++) {
-                    stage(k_full + 8 * (kc % kStages), (kc / kStages) & 1, 52);
+                for (int h = 0; h < T::kParts; h++) {
+                    const unsigned slot = (kc + h) % kStages;
+                    stage(k_full + 8 * slot, ((kc + h) / kStages) & 1, 52);
                     if (!ok) return;
-                    const unsigned hi = desc_lo_sw128(smem_u32(smem + kOffK) + (kc % kStages) * kKStage);
-                    const unsigned lo = hi + (T::kPlaneBytes >> 4), ql = q_lo + h * T::kChunks * (kQChunk >> 4);
-                    const unsigned qh = tmem + kTmemQ + 32 * T::kChunks * h, more = h != 0;
+                    const unsigned hi = planes + slot * (kKStage >> 4), lo = hi + (T::kPlaneBytes >> 4);
+                    const unsigned ql = q_lo + h * T::kChunks * (kQChunk >> 4), qh = tmem + kTmemQ + 32 * T::kChunks * h;
+                    const unsigned more = h != 0;
                     if (elect_one()) {
-                        // the small terms first: each MMA cuts the sum off, relative to what it has come to
 #pragma unroll
                         for (int k = 0; k < 4 * T::kChunks; k++)
                             tc_mma_ts<1>(d, qh + 8 * k, desc_from(lo + (k / 4) * (T::kChunkBytes >> 4) + 2 * (k % 4)), kIdescS,
@@ -446,6 +448,14 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tree_tc(TreeParams p) {
                         for (int k = 0; k < 4 * T::kChunks; k++)
                             tc_mma_ss<1>(d, desc_from(ql + (k / 4) * (kQChunk >> 4) + 2 * (k % 4)),
                                          desc_from(hi + (k / 4) * (T::kChunkBytes >> 4) + 2 * (k % 4)), kIdescS, 1);
+                    }
+                    __syncwarp();
+                }
+#pragma unroll 1
+                for (int h = 0; h < T::kParts; h++, kc++) {
+                    const unsigned hi = planes + (kc % kStages) * (kKStage >> 4);
+                    const unsigned qh = tmem + kTmemQ + 32 * T::kChunks * h;
+                    if (elect_one()) {
 #pragma unroll
                         for (int k = 0; k < 4 * T::kChunks; k++)
                             tc_mma_ts<1>(d, qh + 8 * k, desc_from(hi + (k / 4) * (T::kChunkBytes >> 4) + 2 * (k % 4)), kIdescS, 1);
@@ -689,7 +699,8 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tree_tc(TreeParams p) {
 #pragma unroll
                 for (int k = 0; k < 4; k++) big[k] = fmaxf(big[k], u[e + k]);
             float m_new = fmaxf(fmaxf(big[0], big[1]), fmaxf(big[2], big[3]));
-            m_new = fmaxf(m, fmaf(fmaxf(m_new, meet(i, m_new)), factor, value_power));
+            // (a whole number: what is subtracted is exact then, the same in every tile, and O's corrections are powers of two)
+            m_new = fmaxf(m, rintf(fmaf(fmaxf(m_new, meet(i, m_new)), factor, value_power)));
             const bool fresh = (i * T::kKeys) % kFlushKeys == 0;   // O starts afresh with this tile
             const bool flush = fresh && i > 0;
             const bool move = !fresh && (m_new > m + kThreshold || (m == -INFINITY && m_new > -INFINITY));
