@@ -16,7 +16,8 @@
 // f16 parts need their operands in range whatever the cache holds. So the rows of a tile are scaled by a power of two, K's
 // and V's each by its largest scale (f32: value), and each query row by one of its own. S is multiplied back; the value's
 // power 2^E goes into the weight: w = 2^(s + E - m), where m follows the largest s + E, and the denominator takes w 2^-E.
-// (A row far smaller than its tile's largest has fewer bits: 22 of them down to 2^-10 of it, one fewer for each power below.)
+// Where a tile's rows lie so far apart that its smallest would lose bits (a drafted row that most nodes do not see may hold
+// anything), each of them has a power of its own: rare, and twice the work of the softmax.
 // A K row that is not finite is not a number in the planes, which reaches the rows that see it and no others; a V row that is
 // not finite is zero there, and the weights of those that see it are not a number (a hidden key's weight is 0).
 //
@@ -61,9 +62,10 @@ constexpr int kKStage = 32 * 1024, kVStage = 16 * 1024;
 constexpr int kRawBytes = 3 * 64 * 272;
 constexpr int kFlushKeys = 512;
 constexpr unsigned kSpinLimit = 1u << 22;
-constexpr float kThreshold = 8.0f;               // log2: the reference moves when a weight would exceed 2^8 times it,
-constexpr float kLift = 7.0f;                    // and weights are kept 2^7 times larger: up to 2^15.5, f16's smallest 2^-24
-constexpr int kLeastPower = -100, kMostPower = 100;   // of a tile; smaller values count as 0 (as do zeros)
+constexpr float kThreshold = 5.0f;               // log2: the reference moves when a weight would exceed 2^5 times it,
+constexpr float kLift = 10.0f;                   // and weights are kept 2^10 times larger: up to 2^15.5; f16's last bit, 2^-24,
+                                                 // is then 2^-34 of the reference (2^-22 of weights down to 2^-12 of it)
+constexpr int kLeastPower = -80, kMostPower = 117;   // of a tile or row; smaller values count as 0 (as do zeros)
 
 template <int kType>   // 0 f32, 1 q8_0, 2 q4_0
 struct Shape {
@@ -99,9 +101,11 @@ constexpr int kScouts = 8;
 struct __align__(16) Scout {
     int power;
     unsigned bad[2];   // a bit per row
+    int wide;          // whether the rows have powers of their own
 };
 constexpr int kOffScout = kOffRaw + kRawBytes;             // [K, V][kScouts]
-constexpr int kOffMeet = kOffScout + 2 * kScouts * 16;      // [2][2][128]: the halves of a row meet
+constexpr int kOffPowers = kOffScout + 2 * kScouts * 16;    // [K, V][kScouts][64] bytes: the rows' own powers
+constexpr int kOffMeet = kOffPowers + 2 * kScouts * 64;     // [2][2][128]: the halves of a row meet
 constexpr int kOffRowFac = kOffMeet + 2 * 2 * 128 * 4;     // [128]
 constexpr int kOffSees = kOffRowFac + kRows * 4;           // [128][kTreeWords + 1]
 constexpr int kOffParents = kOffSees + kRows * (kTreeWords + 1) * 4;
@@ -169,10 +173,12 @@ __device__ __forceinline__ void split_pair(float a, float b, unsigned &hi, unsig
 // 2^n for whole n of [-126, 127]
 __device__ __forceinline__ float power(int n) { return __int_as_float((n + 127) << 23); }
 
-// The largest |value| of half of an f32 row, or |scale| of a quantised row, as bits.
+// The largest |value| of half of an f32 row, or |scale| of a quantised row, as bits; `least`: less one, the smallest scale that
+// is not 0 (2^32 - 1: none).
 template <int kType>
-__device__ __forceinline__ unsigned row_most(const unsigned char *row, int half) {
+__device__ __forceinline__ unsigned row_most(const unsigned char *row, int half, unsigned &least) {
     unsigned most = 0;
+    least = 0xffffffffu;
     if constexpr (kType == 0) {
 #pragma unroll 4
         for (int k = 0; k < 32; k++) {
@@ -181,8 +187,11 @@ __device__ __forceinline__ unsigned row_most(const unsigned char *row, int half)
         }
     } else {
 #pragma unroll
-        for (int b = 0; b < 8; b++)
-            most = max(most, (unsigned)(*reinterpret_cast<const unsigned short *>(row + b * (kType == 1 ? 34 : 18)) & 0x7fff));
+        for (int b = 0; b < 8; b++) {
+            const unsigned x = *reinterpret_cast<const unsigned short *>(row + b * (kType == 1 ? 34 : 18)) & 0x7fff;
+            most = max(most, x);
+            least = min(least, x - 1);
+        }
     }
     return most;
 }
@@ -244,6 +253,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tree_tc(TreeParams p) {
     static_assert(T::kRawSlots <= 8 && kScouts == 8 && kBars == 55, "barriers");
     auto scout_bar = [&](bool v, int t) { return scouted + 8 * ((v ? 8 : 0) + (t & 7)); };   // of tile t
     Scout *const scouts = reinterpret_cast<Scout *>(smem + kOffScout);
+    auto powers = [&](bool v, int t) { return reinterpret_cast<signed char *>(smem + kOffPowers) + 64 * ((v ? 8 : 0) + (t & 7)); };
     auto raw_bar = [&](bool v, int i) { return raw_full + 8 * ((v ? 8 : 0) + (i & 7)); };   // of half tile i
     if (warp == 1) {
         for (int i = lane; i < kBars; i += 32) {
@@ -507,8 +517,9 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tree_tc(TreeParams p) {
 #pragma unroll 1
         for (int t = 0; t < n; t++) {
             const int live = tile_rows(t);
-            Scout found = {0, {0, 0}};
-            unsigned most = 0;   // of the rows that are finite
+            Scout found = {0, {0, 0}, 0};
+            unsigned most = 0;                                        // of the rows that are finite:
+            unsigned least = 0xffffffffu, least_scale = 0xffffffffu;  // of those that are not 0, less one
 #pragma unroll 1
             for (int j = 0; j < 2; j++) {
                 const unsigned u = raw_of(is_v, t) + j;
@@ -516,8 +527,8 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tree_tc(TreeParams p) {
                 const unsigned char *const from = smem + kOffRaw + (u % T::kRawSlots) * T::kRawSlot;
                 // f32: a lane has half of a row; quantised: a lane has a row
                 const int r = kType == 0 ? lane & 15 : lane;
-                unsigned mine = 0;
-                if (T::kRawRows * j + r < live) mine = row_most<kType>(from + r * T::kRowPitch, kType == 0 ? lane >> 4 : 0);
+                unsigned mine = 0, small = 0xffffffffu;
+                if (T::kRawRows * j + r < live) mine = row_most<kType>(from + r * T::kRowPitch, kType == 0 ? lane >> 4 : 0, small);
                 if constexpr (kType == 0) mine = max(mine, __shfl_xor_sync(0xffffffffu, mine, 16));
                 const bool bad = mine >= (kType == 0 ? 0x7f800000u : 0x7c00u);
                 const unsigned bits = __ballot_sync(0xffffffffu, bad);
@@ -525,10 +536,27 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tree_tc(TreeParams p) {
                     found.bad[0] |= (bits & 0xffff) << (16 * j);
                 else
                     found.bad[j] = bits;
-                if (!bad) most = max(most, mine);
+                if (!bad) {
+                    most = max(most, mine);
+                    least = min(least, mine - 1);
+                    least_scale = min(least_scale, small);
+                }
+                powers(is_v, t)[T::kRawRows * j + r] = (signed char)power_of<kType>(bad ? 0 : mine);
                 if (lane == 0) mbar_arrive(raw_empty + 8 * (u % T::kRawSlots));
             }
-            found.power = power_of<kType>(__reduce_max_sync(0xffffffffu, most));
+            most = __reduce_max_sync(0xffffffffu, most);
+            least = __reduce_min_sync(0xffffffffu, least);
+            found.power = power_of<kType>(most);
+            // Against f16's 2^-24 a scale of [8, 16) has 17 powers to spare until a product loses a bit, the largest value of an
+            // f32 row, of [2^10, 2^11), has 12 until fewer than 22 are left. A tile of V whose power is that of a row that a
+            // query hardly sees costs the weights of the other tiles as many bits: 7 at most.
+            const int spread = least < most ? found.power - power_of<kType>(least + 1) : 0;
+            found.wide = spread > (is_v ? 7 : 12);
+            if (kType != 0) {
+                least_scale = __reduce_min_sync(0xffffffffu, least_scale);
+                if (least_scale < most && found.power - power_of<kType>(least_scale + 1) > 17) found.wide = 1;
+            }
+            __syncwarp();   // the rows' powers
             if (lane == 0) {
                 scouts[(is_v ? kScouts : 0) + (t & 7)] = found;
                 mbar_arrive(scout_bar(is_v, t));
@@ -564,7 +592,8 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tree_tc(TreeParams p) {
                 const unsigned full = (is_v ? v_full : k_full) + 8 * (c % kStages);
                 const unsigned char *const raw_row = smem + kOffRaw + ((u0 + j) % T::kRawSlots) * T::kRawSlot + row * T::kRowPitch;
                 const bool bad = (key < 32 ? known.bad[0] : known.bad[1]) >> (key & 31) & 1;
-                const float by = key < live && !bad ? scale_by : 0.0f;
+                float by = key < live && !bad ? scale_by : 0.0f;
+                if (known.wide && by != 0.0f) by = power(-powers(is_v, t)[key]);
                 unsigned hi[16], lo[16];
                 if constexpr (kType == 0) {
                     // (an odd block's halves are swapped: eight lanes' words fall into different banks)
@@ -627,7 +656,8 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tree_tc(TreeParams p) {
         const unsigned lane_at = tmem + ((unsigned)((warp & 3) * 32) << 16);
         const float row_factor = reinterpret_cast<const float *>(smem + kOffRowFac)[r];
         const bool live = r < rows, whole = it.runs == 1;
-        float m = -INFINITY, l = 0.0f, m_out = -INFINITY;   // m_out: the reference of what is in memory already
+        // m_out: the reference of what is in memory already, which is at most 2^30 above it
+        float m = -INFINITY, l = 0.0f, m_out = -INFINITY;
         // the other half's value of the row (the warps w and w + 4 meet)
         auto meet = [&](int x, float mine) {
             float *const buf = reinterpret_cast<float *>(smem + kOffMeet) + (x & 1) * 256;
@@ -638,8 +668,8 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tree_tc(TreeParams p) {
         // dims of column group j (32 columns) of this thread's half of O
         auto dims_of = [&](int j) { return kType == 0 ? 128 * half + 32 * j : 32 * T::block(half, j); };
         const bool idle = 32 * (warp & 3) >= rows;   // (no row of this warp is live: nothing reads its lanes)
-        // Values' powers are taken relative to that of the run's first tile: the exponents of the weights stay as small as
-        // the scores, to whose rounding they would add. (Within [-20, 16], which keeps the differences in range.)
+        // Values' powers are taken relative to that of the run's first tile, within [-9, 8]: then no weight's share of the
+        // denominator, w 2^-E, leaves f32's range, for E of [-80, 117].
         int power0 = 0;
         float *const flushed = p.part_acc + ((size_t)blockIdx.x * kRows * (kD / 4) + r) * 4;   // [64 x four dims][128 rows]
 #pragma unroll 1
@@ -654,9 +684,11 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tree_tc(TreeParams p) {
             wait(scout_bar(false, i), (i >> 3) & 1, 58);
             wait(scout_bar(true, i), (i >> 3) & 1, 58);
             const Scout known = scouts[kScouts + (i & 7)];
-            if (i == 0) power0 = min(max(known.power, -20), 16);
-            const float value_power = (float)(known.power - power0), value_inverse = power(power0 - known.power);
-            float factor = row_factor * power(scouts[i & 7].power);   // of S; > 0, so that a hidden row's -inf stays that
+            if (i == 0) power0 = min(max(known.power, -9), 8);
+            float value_power = (float)(known.power - power0), value_inverse = power(power0 - known.power);
+            const Scout known_k = scouts[i & 7];
+            const bool wide = (known.wide | known_k.wide) != 0;
+            float factor = row_factor * power(known_k.power);   // of S; > 0, so that a hidden row's -inf stays that
             if (factor < 1e-30f) factor = 1e-30f;
             __syncwarp();
             tc_fence_after();
@@ -670,6 +702,28 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tree_tc(TreeParams p) {
                 tmem_ld16(s_at, u);
             }
             const int key0 = lo_key + i * T::kKeys + T::kHalf * half;
+            // The powers of this half's rows, four at a time: K's, and V's less power0
+            auto own_powers = [&](bool v, int e, int (&own)[4]) {
+                const char4 four = reinterpret_cast<const char4 *>(powers(v, i) + T::kHalf * half)[e / 4];
+                const Scout of = scouts[(v ? kScouts : 0) + (i & 7)];
+                const bool each = of.wide != 0;
+                const int all = of.power, less = v ? power0 : 0;
+                own[0] = (each ? four.x : all) - less;
+                own[1] = (each ? four.y : all) - less;
+                own[2] = (each ? four.z : all) - less;
+                own[3] = (each ? four.w : all) - less;
+            };
+            if (__builtin_expect(wide, 0)) {
+#pragma unroll
+                for (int e = 0; e < T::kHalf; e += 4) {
+                    int own[4];
+                    own_powers(false, e, own);
+#pragma unroll
+                    for (int k = 0; k < 4; k++) u[e + k] *= row_factor * power(own[k]);
+                }
+                factor = 1.0f;
+                value_power = value_inverse = 0.0f;
+            }
             if ((known.bad[0] | known.bad[1]) != 0) {   // rare: a V row that is not finite
                 const unsigned bits = T::kHalf == 32 ? known.bad[half] : known.bad[0] >> (16 * half);
 #pragma unroll
@@ -698,6 +752,15 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tree_tc(TreeParams p) {
             for (int e = 4; e < T::kHalf; e += 4)
 #pragma unroll
                 for (int k = 0; k < 4; k++) big[k] = fmaxf(big[k], u[e + k]);
+            if (__builtin_expect(wide, 0)) {
+#pragma unroll
+                for (int e = 0; e < T::kHalf; e += 4) {
+                    int own[4];
+                    own_powers(true, e, own);
+#pragma unroll
+                    for (int k = 0; k < 4; k++) big[k] = e == 0 ? u[k] + own[k] : fmaxf(big[k], u[e + k] + own[k]);
+                }
+            }
             float m_new = fmaxf(fmaxf(big[0], big[1]), fmaxf(big[2], big[3]));
             // (a whole number: what is subtracted is exact then, the same in every tile, and O's corrections are powers of two)
             m_new = fmaxf(m, rintf(fmaf(fmaxf(m_new, meet(i, m_new)), factor, value_power)));
@@ -710,9 +773,19 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tree_tc(TreeParams p) {
                 tc_fence_after();
             }
             if (flush) {
-                // O, relative to m, is added to what is in memory (or takes its place, where that is nothing beside it);
-                // a warp's 32 rows lie together there
-                const bool over = m_out == -INFINITY || m > m_out + 60.0f;
+                // O, relative to m, is added to what is in memory, relative to m_out (or takes its place, where that is nothing
+                // beside it); a warp's 32 rows lie together there
+                const bool over = m_out == -INFINITY || m > m_out + 90.0f;
+                if (!over && m > m_out + 30.0f && live && !*wait.abort) {   // rare
+                    const float down = exp2f(m_out - m);
+#pragma unroll 1
+                    for (int j = 0; j < 32; j++) {
+                        float4 *const at = reinterpret_cast<float4 *>(flushed + (size_t)(32 * half + j) * (kRows * 4));
+                        const float4 x = __ldcg(at);
+                        *at = make_float4(x.x * down, x.y * down, x.z * down, x.w * down);
+                    }
+                    m_out = m;
+                }
                 const float g = over ? 1.0f : exp2f(m - m_out);
 #pragma unroll 1
                 for (int j = 0; j < 4; j++) {
@@ -752,7 +825,20 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tree_tc(TreeParams p) {
                 l *= corr;
                 m = m_new;
             }
-            const float shift = value_power - ((m == -INFINITY ? 0.0f : m) - kLift);
+            float shift = value_power - ((m == -INFINITY ? 0.0f : m) - kLift);
+            if (__builtin_expect(wide, 0)) {   // the denominator's terms, and each weight's own exponent
+#pragma unroll
+                for (int e = 0; e < T::kHalf; e += 4) {
+                    int own[4];
+                    own_powers(true, e, own);
+#pragma unroll
+                    for (int k = 0; k < 4; k++) {
+                        l += ex2(u[e + k] + shift);
+                        u[e + k] += (float)own[k] + shift;
+                    }
+                }
+                shift = 0.0f;
+            }
             float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
             for (int e0 = 0; e0 < T::kHalf; e0 += 16) {   // per 16 keys: eight words of hi, eight of lo
@@ -787,7 +873,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tree_tc(TreeParams p) {
             // (O lacks the power that the values' are relative to)
             const float inv = whole ? power(power0) / l : power(power0);
             // part of the row may be in memory; where the last part outweighs that past all bounds, it is dropped
-            const bool join = m_out != -INFINITY && m <= m_out + 60.0f;
+            const bool join = m_out != -INFINITY && m <= m_out + 90.0f;
             const float g = join ? exp2f(m_out - m) : 0.0f;
 #pragma unroll 1
             for (int j = 0; j < 4; j++) {

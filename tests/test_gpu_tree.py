@@ -178,6 +178,114 @@ def test_rows_that_are_not_seen_may_hold_anything(dim, kv_dtype, value):
     assert (got[4:] == CANARY).all()
 
 
+@pytest.mark.parametrize("dim", [64, 256])
+@pytest.mark.parametrize("kv_dtype,value", [(0, 3e38), (0, -1e30), (0, 1e7), (1, 65504.0), (1, -900.0), (2, 65504.0)])
+def test_rows_that_are_not_seen_may_be_of_any_size(dim, kv_dtype, value):
+    """As above, with finite values: nodes 0 and 1 keep all their bits beside a row 2^20 and more times theirs."""
+    shapes = [(90, 4, [-1, 0, 0, 2])]
+    step = Step(3, kv_dtype, shapes, 6, heads=4, kv=2, dim=dim, stride=120)
+    for which in (0, 1):
+        for row in [92] + list(range(94, 120)):
+            _spoil(step, which, 0, row, value)
+    step.upload()
+    step.call()
+    got = step.out.cpu().numpy().reshape(6, 4, dim)
+    want, bound = R.attention(step.caches, 0, 90, 2, shapes[0][2], step.q[0].reshape(6, 4, dim), 4, step.scale)
+    assert (np.abs(got[:2] - want) <= bound).all()
+    assert (got[4:] == CANARY).all()
+
+
+@pytest.mark.parametrize("heads,kv,base", [(4, 2, 300), (8, 1, 3000)])
+@pytest.mark.parametrize("kv_dtype", [0, 1, 2], ids=["f32", "q8", "q4"])
+@pytest.mark.parametrize("keys,values", [(24, 0), (0, 24), (20, 20)])
+def test_rows_of_very_different_size_side_by_side(heads, kv, base, kv_dtype, keys, values):
+    """Rows between their full size and 2^-keys (2^-values) of it, at random along the cache; some are 0."""
+    shapes = [(base, 5, R.random_tree(np.random.default_rng(1), 5)), (base // 2, 3, R.chain(3))]
+    step = Step(13, kv_dtype, shapes, 5, heads=heads, kv=kv)
+    rng = np.random.default_rng(14)
+    for s, (b, live, _) in enumerate(shapes):
+        for which, spread in ((0, keys), (1, values)):
+            size = 2.0 ** (-spread * rng.random((kv, b + live, 1)))
+            size[rng.random(size.shape) < 0.05] = 0.0
+            step.caches.put(which, s, 0, rng.standard_normal((kv, b + live, 256)) * size)
+    step.upload()
+    step.run()
+
+
+def test_f32_rows_of_every_size_side_by_side():
+    """Keys of 2^-60 .. 2^60 (their signs make the scores of the large ones -infinity's neighbours), values of 2^-60 .. 2^60."""
+    shapes = [(200, 5, R.chain(5))]
+    step = Step(15, 0, shapes, 5, heads=4, kv=2)
+    rng = np.random.default_rng(16)
+    step.q[:] = np.abs(step.q)
+    k = -np.abs(rng.standard_normal((2, 205, 256))) * 2.0 ** rng.integers(-60, 61, (2, 205, 1))
+    step.caches.put(0, 0, 0, k)
+    step.caches.put(1, 0, 0, rng.standard_normal((2, 205, 256)) * 2.0 ** rng.integers(-60, 61, (2, 205, 1)))
+    step.upload()
+    step.run()
+
+
+@pytest.mark.parametrize("kv_dtype", [0, 1, 2], ids=["f32", "q8", "q4"])
+@pytest.mark.parametrize("base", [1500, 5000, 9000])
+def test_long_runs_of_one_slot_each(kv_dtype, base):
+    """So many slots that a CTA takes 1,500 rows and more in one run: the sums leave the tensor cores' registers on the way."""
+    rng = np.random.default_rng(base)
+    slots = 40 if base == 1500 else 16
+    shapes = [(base + int(rng.integers(0, 70)), 3, R.random_tree(rng, 3)) for _ in range(slots)]
+    step = Step(base, kv_dtype, shapes, 3, heads=4, kv=4 if base == 1500 else 1)
+    step.run()
+
+
+def test_long_runs_with_scores_that_fall_and_rise():
+    """The largest score comes early, in the middle or late in a long run (what lies in memory outweighs the rest or is outweighed)."""
+    slots, base = 40, 2000
+    shapes = [(base, 3, R.chain(3))] * slots
+    step = Step(17, 1, shapes, 3, heads=4, kv=4)
+    rng = np.random.default_rng(18)
+    direction = np.sign(rng.standard_normal(256))
+    x = np.arange(base + 3)
+    for s in range(slots):
+        peak = (s + 0.5) / slots * (base + 3)
+        size = 12.0 * (1.0 - np.abs(x - peak) / (base + 3))
+        step.caches.put(0, s, 0, np.broadcast_to(size[:, None] * direction, (4, base + 3, 256))
+                        + 0.3 * rng.standard_normal((4, base + 3, 256)))
+    step.q[:] = np.tile(direction, 4) + 0.1 * rng.standard_normal(step.q.shape)
+    step.upload()
+    step.run()
+
+
+@pytest.mark.parametrize("dim", [64, 256])
+@pytest.mark.parametrize("scale", [0.0, -0.05, 3.0])
+def test_scales_of_any_sign(dim, scale):
+    shapes = [(400, 9, R.random_tree(np.random.default_rng(3), 9))]
+    step = Step(19, 1, shapes, 9, heads=4, kv=2, dim=dim)
+    step.scale = scale
+    step.call()
+    got = step.out.cpu().numpy().reshape(9, 4, dim)
+    # (the bound's parts that go with the scores take the scale's size)
+    want, _ = R.attention(step.caches, 0, 400, 9, shapes[0][2], step.q[0].reshape(9, 4, dim), 4, scale)
+    _, bound = R.attention(step.caches, 0, 400, 9, shapes[0][2], np.sign(scale) * step.q[0].reshape(9, 4, dim), 4, abs(scale))
+    assert (np.abs(got - want) <= bound).all()
+
+
+@pytest.mark.parametrize("dim", [64, 256])
+@pytest.mark.parametrize("value", [float("nan"), float("inf")])
+def test_queries_that_are_not_finite(dim, value):
+    """They are not a number in their own head and node alone."""
+    shapes = [(130, 5, R.chain(5))]
+    step = Step(20, 1, shapes, 5, heads=4, kv=2, dim=dim)
+    clean = step.q.copy()
+    step.q.reshape(5, 4, dim)[3, 1, 7] = value
+    step.upload()
+    step.call()
+    got = step.out.cpu().numpy().reshape(5, 4, dim)
+    want, bound = R.attention(step.caches, 0, 130, 5, shapes[0][2], clean[0].reshape(5, 4, dim), 4, step.scale)
+    others = np.ones((5, 4), dtype=bool)
+    others[3, 1] = False
+    assert not np.isfinite(got[3, 1]).any()
+    assert (np.abs(got - want) <= bound)[others].all()
+
+
 @pytest.mark.parametrize("kv_dtype", [0, 1, 2], ids=["f32", "q8", "q4"])
 @pytest.mark.parametrize("k_scale,v_scale", [(1e-3, 1e-4), (30.0, 3000.0), (1.0, 1e-3), (1e-4, 2e4)])
 def test_small_and_large_values(kv_dtype, k_scale, v_scale):
@@ -443,6 +551,34 @@ def test_rejections_that_leave_nothing():
     draft = np.full((1, 4, 64), 0.9, dtype=np.float32)
     for u in ([0.3, 0.9, 0.9, 0.9], [0.3, 0.9, 0.9, 0.1]):
         _verify([R.star(4)], [[0, 9, 9, 10]], target, draft, np.array([u], dtype=np.float32), [4])
+
+
+@pytest.mark.parametrize("slots,vocab", [(1, 151936), (3, 50257), (12, 4099), (40, 1000)])
+@pytest.mark.parametrize("looked_up", [False, True], ids=["drawn", "looked up"])
+def test_many_rejections_in_a_row(looked_up, slots, vocab):
+    """Every child of a wide tree is refused (its token's probability is next to nothing, or taken before)."""
+    rng = np.random.default_rng(vocab)
+    nodes = 12
+    _, _, target, draft, u = _drafted(rng, slots, nodes, vocab, 3, near=1.5)
+    parents = [R.star(nodes) if s % 2 == 0 else [-1] + [0] * 5 + [1] * (nodes - 6) for s in range(slots)]
+    # the root's tokens: some of the most probable ones, some twice
+    tokens = []
+    for s in range(slots):
+        order = np.argsort(-target[s, 0])
+        tokens.append([0] + [int(order[j % 7]) for j in range(nodes - 1)])
+    u[:, 1:] = 1.0 - 2.0 ** -24
+    _verify(parents, tokens, target, None if looked_up else draft, u, [nodes] * slots)
+
+
+def test_rejected_tokens_that_hold_nearly_all():
+    """Looked-up tokens take all but some 2^-20 of the mass away: what is left is summed anew, not taken off."""
+    nodes, vocab = 6, 5000
+    target = np.full((1, nodes, vocab), 2.0 ** -33, dtype=np.float32)
+    target[0, :, 100:105] = [0.5, 0.25, 0.125, 0.0625, 0.0625]
+    tokens = [[0, 100, 101, 102, 103, 104]]
+    for u0 in (0.0, 0.3, 0.999):
+        u = np.array([[u0] + [1.0 - 2.0 ** -24] * (nodes - 1)], dtype=np.float32)
+        _, count, _ = _verify([R.star(nodes)], tokens, target, None, u, [nodes])
 
 
 def test_siblings_with_the_same_token():

@@ -75,7 +75,13 @@ def attention(caches, slot, base, live, parents, q, heads, scale):
     which is rounded (2^-22 of the value, and the product of the two remainders 2^-22): a score's error is at most
     (2^-22 + 2 * 2^-22 + (3 * 16 + 8) u) * scale * sum |q k|, for 16 steps of three products each; one of 2^-22 of the score
     comes from the exponential's argument. Weights are off by that and by 2^-21 (the exponential); the sums over n rows by
-    (3 n / 16 + 64) u of the sum of the weights times |v|, and the folds of the runs by another 64 u."""
+    (3 n / 16 + 64) u of the sum of the weights times |v|, and the folds of the runs by another 64 u.
+
+    Weights are not exact to 2^-22 of themselves however small they are. Their last bit is f16's 2^-24, they are kept 2^10
+    times 2^(s + E - m), and m is at most the largest s + E and one half; so row j's weight is off by 2^-25 - 10 + 1/2 of
+    2^(max (s + E)), its values, below 2^(E_j + 11) each, are multiplied back by 2^-E_j, and a tile's E is at most 7 above
+    that of any of its rows, whose largest value is 2^(E + 10) or more: altogether less than 2^-35 + 1/2 + 7 + 1 of the largest
+    p_j max |v_j| per row, n 2^-26 of it."""
     kv, dim = caches.kv, caches.dim
     group = heads // kv
     out, bound = np.zeros((live, heads, dim)), np.zeros((live, heads, dim))
@@ -92,6 +98,7 @@ def attention(caches, slot, base, live, parents, q, heads, scale):
             out[i, h] = p @ v
             most = off.max()   # (of a weight and of the whole: twice)
             bound[i, h] = (2 * most + 2.0 ** -20 + (3 * len(rows) / 16 + 128) * u) * (p @ np.abs(v))
+            bound[i, h] += len(rows) * 2.0 ** -26 * (p * np.abs(v).max(1)).max()
     return out, bound
 
 
