@@ -104,8 +104,8 @@ struct __align__(16) Scout {
     int wide;          // whether the rows have powers of their own
 };
 constexpr int kOffScout = kOffRaw + kRawBytes;             // [K, V][kScouts]
-constexpr int kOffPowers = kOffScout + 2 * kScouts * 16;    // [K, V][kScouts][64] bytes: the rows' own powers
-constexpr int kOffMeet = kOffPowers + 2 * kScouts * 64;     // [2][2][128]: the halves of a row meet
+constexpr int kOffFactors = kOffScout + 2 * kScouts * 16;   // [K, V][kScouts][64]: what each row is multiplied by
+constexpr int kOffMeet = kOffFactors + 2 * kScouts * 64 * 4;   // [2][2][128]: the halves of a row meet
 constexpr int kOffRowFac = kOffMeet + 2 * 2 * 128 * 4;     // [128]
 constexpr int kOffSees = kOffRowFac + kRows * 4;           // [128][kTreeWords + 1]
 constexpr int kOffParents = kOffSees + kRows * (kTreeWords + 1) * 4;
@@ -253,7 +253,8 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tree_tc(TreeParams p) {
     static_assert(T::kRawSlots <= 8 && kScouts == 8 && kBars == 55, "barriers");
     auto scout_bar = [&](bool v, int t) { return scouted + 8 * ((v ? 8 : 0) + (t & 7)); };   // of tile t
     Scout *const scouts = reinterpret_cast<Scout *>(smem + kOffScout);
-    auto powers = [&](bool v, int t) { return reinterpret_cast<signed char *>(smem + kOffPowers) + 64 * ((v ? 8 : 0) + (t & 7)); };
+    // of tile t, by row: a power of two, 0 where there is no row, not a number where the row is not finite
+    auto factors = [&](bool v, int t) { return reinterpret_cast<float *>(smem + kOffFactors) + 64 * ((v ? 8 : 0) + (t & 7)); };
     auto raw_bar = [&](bool v, int i) { return raw_full + 8 * ((v ? 8 : 0) + (i & 7)); };   // of half tile i
     if (warp == 1) {
         for (int i = lane; i < kBars; i += 32) {
@@ -541,7 +542,10 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tree_tc(TreeParams p) {
                     least = min(least, mine - 1);
                     least_scale = min(least_scale, small);
                 }
-                powers(is_v, t)[T::kRawRows * j + r] = (signed char)power_of<kType>(bad ? 0 : mine);
+                if (kType != 0 || lane < 16)
+                    factors(is_v, t)[T::kRawRows * j + r] = bad ? __int_as_float(0x7fffffff)
+                                                            : T::kRawRows * j + r < live ? power(-power_of<kType>(mine))
+                                                                                         : 0.0f;
                 if (lane == 0) mbar_arrive(raw_empty + 8 * (u % T::kRawSlots));
             }
             most = __reduce_max_sync(0xffffffffu, most);
@@ -556,7 +560,13 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tree_tc(TreeParams p) {
                 least_scale = __reduce_min_sync(0xffffffffu, least_scale);
                 if (least_scale < most && found.power - power_of<kType>(least_scale + 1) > 17) found.wide = 1;
             }
-            __syncwarp();   // the rows' powers
+            if (!found.wide) {   // one power for all
+                for (int k = lane; k < T::kKeys; k += 32) {
+                    float *const by = factors(is_v, t) + k;
+                    if (*by > 0.0f) *by = power(-found.power);
+                }
+            }
+            __syncwarp();
             if (lane == 0) {
                 scouts[(is_v ? kScouts : 0) + (t & 7)] = found;
                 mbar_arrive(scout_bar(is_v, t));
@@ -582,8 +592,6 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tree_tc(TreeParams p) {
             wait(raw_bar(is_v, 2 * t), ((2 * t) >> 3) & 1, 56);
             wait(raw_bar(is_v, 2 * t + 1), ((2 * t + 1) >> 3) & 1, 56);
             wait(scout_bar(is_v, t), (t >> 3) & 1, 58);
-            const Scout known = scouts[(is_v ? kScouts : 0) + (t & 7)];
-            const float scale_by = power(-known.power);
             // K: both halves of a part, then the other part; V: both parts of a half, then the other half
 #pragma unroll 1
             for (int s = 0; s < 2 * T::kParts; s++) {
@@ -591,9 +599,9 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tree_tc(TreeParams p) {
                 const int key = T::kRawRows * j + row;
                 const unsigned full = (is_v ? v_full : k_full) + 8 * (c % kStages);
                 const unsigned char *const raw_row = smem + kOffRaw + ((u0 + j) % T::kRawSlots) * T::kRawSlot + row * T::kRowPitch;
-                const bool bad = (key < 32 ? known.bad[0] : known.bad[1]) >> (key & 31) & 1;
-                float by = key < live && !bad ? scale_by : 0.0f;
-                if (known.wide && by != 0.0f) by = power(-powers(is_v, t)[key]);
+                float by = factors(is_v, t)[key];
+                const bool bad = by != by;
+                if (bad) by = 0.0f;
                 unsigned hi[16], lo[16];
                 if constexpr (kType == 0) {
                     // (an odd block's halves are swapped: eight lanes' words fall into different banks)
@@ -702,28 +710,6 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tree_tc(TreeParams p) {
                 tmem_ld16(s_at, u);
             }
             const int key0 = lo_key + i * T::kKeys + T::kHalf * half;
-            // The powers of this half's rows, four at a time: K's, and V's less power0
-            auto own_powers = [&](bool v, int e, int (&own)[4]) {
-                const char4 four = reinterpret_cast<const char4 *>(powers(v, i) + T::kHalf * half)[e / 4];
-                const Scout of = scouts[(v ? kScouts : 0) + (i & 7)];
-                const bool each = of.wide != 0;
-                const int all = of.power, less = v ? power0 : 0;
-                own[0] = (each ? four.x : all) - less;
-                own[1] = (each ? four.y : all) - less;
-                own[2] = (each ? four.z : all) - less;
-                own[3] = (each ? four.w : all) - less;
-            };
-            if (__builtin_expect(wide, 0)) {
-#pragma unroll
-                for (int e = 0; e < T::kHalf; e += 4) {
-                    int own[4];
-                    own_powers(false, e, own);
-#pragma unroll
-                    for (int k = 0; k < 4; k++) u[e + k] *= row_factor * power(own[k]);
-                }
-                factor = 1.0f;
-                value_power = value_inverse = 0.0f;
-            }
             if ((known.bad[0] | known.bad[1]) != 0) {   // rare: a V row that is not finite
                 const unsigned bits = T::kHalf == 32 ? known.bad[half] : known.bad[0] >> (16 * half);
 #pragma unroll
@@ -747,20 +733,34 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tree_tc(TreeParams p) {
                 for (int e = 0; e < T::kHalf; e++)
                     if (!(sees >> e & 1)) u[e] = -INFINITY;
             }
+            // Rows with powers of their own: u becomes s + E here, and the denominator's terms are summed relative to their own
+            // largest. (The sums are rounded where they are exact otherwise: 2^-24 of the exponent, which a spread of 2^20 takes
+            // to some 30.)
+            float most_s = -INFINITY, sum_s = 0.0f;
+            if (__builtin_expect(wide, 0)) {
+                const float *const by_k = factors(false, i) + T::kHalf * half, *const by_v = factors(true, i) + T::kHalf * half;
+                auto power_in = [](float by) { return 127 - (__float_as_int(by) >> 23); };
+#pragma unroll
+                for (int e = 0; e < T::kHalf; e++) {
+                    const float f = row_factor * power(power_in(by_k[e]));
+                    u[e] *= f < 1e-30f ? 1e-30f : f;
+                    most_s = fmaxf(most_s, u[e]);
+                }
+                if (most_s > -INFINITY) {
+#pragma unroll
+                    for (int e = 0; e < T::kHalf; e++) {
+                        sum_s += ex2(u[e] - most_s);
+                        u[e] += (float)(power_in(by_v[e]) - power0);
+                    }
+                }
+                factor = 1.0f;
+                value_power = value_inverse = 0.0f;
+            }
             float big[4] = {u[0], u[1], u[2], u[3]};
 #pragma unroll
             for (int e = 4; e < T::kHalf; e += 4)
 #pragma unroll
                 for (int k = 0; k < 4; k++) big[k] = fmaxf(big[k], u[e + k]);
-            if (__builtin_expect(wide, 0)) {
-#pragma unroll
-                for (int e = 0; e < T::kHalf; e += 4) {
-                    int own[4];
-                    own_powers(true, e, own);
-#pragma unroll
-                    for (int k = 0; k < 4; k++) big[k] = e == 0 ? u[k] + own[k] : fmaxf(big[k], u[e + k] + own[k]);
-                }
-            }
             float m_new = fmaxf(fmaxf(big[0], big[1]), fmaxf(big[2], big[3]));
             // (a whole number: what is subtracted is exact then, the same in every tile, and O's corrections are powers of two)
             m_new = fmaxf(m, rintf(fmaf(fmaxf(m_new, meet(i, m_new)), factor, value_power)));
@@ -825,20 +825,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tree_tc(TreeParams p) {
                 l *= corr;
                 m = m_new;
             }
-            float shift = value_power - ((m == -INFINITY ? 0.0f : m) - kLift);
-            if (__builtin_expect(wide, 0)) {   // the denominator's terms, and each weight's own exponent
-#pragma unroll
-                for (int e = 0; e < T::kHalf; e += 4) {
-                    int own[4];
-                    own_powers(true, e, own);
-#pragma unroll
-                    for (int k = 0; k < 4; k++) {
-                        l += ex2(u[e + k] + shift);
-                        u[e + k] += (float)own[k] + shift;
-                    }
-                }
-                shift = 0.0f;
-            }
+            const float shift = value_power - ((m == -INFINITY ? 0.0f : m) - kLift);
             float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
             for (int e0 = 0; e0 < T::kHalf; e0 += 16) {   // per 16 keys: eight words of hi, eight of lo
@@ -856,6 +843,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tree_tc(TreeParams p) {
                 tmem_st16(s_at + e0, o);
             }
             l = fmaf((sum[0] + sum[1]) + (sum[2] + sum[3]), value_inverse, l);
+            if (sum_s != 0.0f) l = fmaf(sum_s, exp2f(most_s - m + kLift), l);
             tmem_wait_st();
             tc_fence_before();
             __syncwarp();
