@@ -474,6 +474,8 @@ int hipml_attn_chunk_staged_gated(hipml_stream_t stream, const float *q, float *
  * Attention of the drafted nodes in one call: node i sees cache rows [0, base), its own row and
  * those of its ancestors. q and out are f32 [slots][nodes][n_heads*head_dim], 16-byte aligned. A row
  * that a node does not see may hold anything, NaN and infinities too, without effect on it.
+ * Where it sees a row that is not finite, the heads of that KV head are not finite; rows of f32 caches
+ * below 2^-70 lose bits.
  * workspace: hipml_attn_tree_workspace_bytes(...) bytes on 16 (0: the arguments are refused; it
  * depends on the current device's SMs). */
 size_t hipml_attn_tree_workspace_bytes(int n_heads, int n_kv, int head_dim, int nodes, int slots);
