@@ -17,7 +17,7 @@
 // and V's each by its largest scale (f32: value), and each query row by one of its own. S is multiplied back; the value's
 // power 2^E goes into the weight: w = 2^(s + E - m), where m follows the largest s + E, and the denominator takes w 2^-E.
 // Where a tile's rows lie so far apart that its smallest would lose bits (a drafted row that most nodes do not see may hold
-// anything), each of them has a power of its own: rare, and twice the work of the softmax.
+// anything), each of them has a power of its own (rare; 64 nodes over 100,000 rows with every tile so: 517 us instead of 490).
 // A K row that is not finite is not a number in the planes, which reaches the rows that see it and no others; a V row that is
 // not finite is zero there, and the weights of those that see it are not a number (a hidden key's weight is 0).
 //

@@ -11,10 +11,11 @@
 // A slot is one cluster of CTAs; each has a part of the vocabulary, each warp a run of that. What the walk asks of single
 // tokens, r(x) and q(x) of every node, is fetched by all nodes at once in the beginning (one trip to memory instead of one
 // per level). A rejected child costs one pass over the target and the draft row, all CTAs together; without draft rows only
-// the first one of a node does, the others take their token's probability off the sum. The sums of the last pass are those by
-// which the next token is found (another one where it was not over all that was rejected). Differences, sums and comparisons
-// are in 64 bits: over 150,000 probabilities a 32-bit running sum moves some thousandth of the drawn tokens by one place. r
-// after the second and later rejections is computed from the rows again, so nothing is kept per probability.
+// the first one of a node does: it leaves out the tokens of all its children, what was not tried yet is added back, and if
+// the walk ends there these are the sums that it needs. The sums of the last pass are those by which the next token is found.
+// Differences, sums and comparisons are in 64 bits: over 150,000 probabilities a 32-bit running sum moves some thousandth of
+// the drawn tokens by one place. r after the second and later rejections is computed from the rows again, so nothing is kept
+// per probability.
 #include <atomic>
 
 #include "sm100_ptx.cuh"
@@ -61,6 +62,9 @@ __global__ void __launch_bounds__(kThreads) tree_verify(VerifyParams p) {
     __shared__ int s_parent[kTreeNodes], s_token[kTreeNodes];
     __shared__ float s_u[kTreeNodes], s_p[kTreeNodes], s_q[kTreeNodes];
     __shared__ Left s_left;
+    // without draft rows: a child's probability where its token is first tried, else 0; the sum of those of the children behind
+    __shared__ float s_c[kTreeNodes];
+    __shared__ double s_after[kTreeNodes];
     __shared__ double s_sum[2];               // this CTA's part of a pass, read by the others (the passes take turns)
     __shared__ double s_all[kCtas];           // the sums of the parts
     __shared__ double s_warp[kWarps];         // of this part, by warp
@@ -111,11 +115,9 @@ __global__ void __launch_bounds__(kThreads) tree_verify(VerifyParams p) {
         }
         return r;
     };
-    // One pass over the row: the sums of the warps' runs, and the sum of all (everywhere the same bits). `known`: how many of
-    // the rejections the runs' sums have in them already (-1: they are of another row); without draft rows only runs that
-    // have lost a token since are summed again.
+    // One pass over the row: the sums of the warps' runs, and the sum of all (everywhere the same bits).
     int passes = 0;
-    auto pass = [&](int tried, int known) {
+    auto pass = [&](int tried) {
         const float *const target = p.target + (long long)(first + here) * p.row_stride;
         const float *const draft = p.draft && tried > 0 ? p.draft + (long long)(first + here) * p.row_stride : nullptr;
         const int w0 = min(v0 + warp * run, v1), w1 = min(w0 + run, v1);
@@ -123,13 +125,8 @@ __global__ void __launch_bounds__(kThreads) tree_verify(VerifyParams p) {
         // an eighth of the instructions in 64 bits. (The loops are loops: this code runs once or twice a launch, and its
         // lines come from beyond the instruction cache: unrolled in 64 bits 8 nodes of 151,936 took 30 us, so 12. Sixteen
         // values at once take 80 registers, which leaves an SM one CTA: 32 slots of 8 nodes 62 us, with eight 32.)
-        bool again = p.draft || known < 0;
-        if (!again)
-            for (int j = known; j < tried; j++) again = again || (s_left.token[j] >= w0 && s_left.token[j] < w1);
         double sum = 0.0;
-        if (!again) {
-            sum = lane == 0 ? s_warp[warp] : 0.0;
-        } else if (!p.draft || tried <= 1) {
+        if (!p.draft || tried <= 1) {
             LongSum s;
 #pragma unroll 1
             for (int x0 = w0 + lane; x0 < w1; x0 += 32 * kAtOnce) {
@@ -151,11 +148,19 @@ __global__ void __launch_bounds__(kThreads) tree_verify(VerifyParams p) {
                     }
                 }
 #pragma unroll
-                for (int k = 0; k < kAtOnce; k++) {
-                    const float u = a[k] > 0.0f && a[k] < INFINITY ? a[k] : 0.0f;   // as probability()
-                    const float v = b[k] > 0.0f && b[k] < INFINITY ? b[k] : 0.0f;
-                    const float d = u - v, e = d - u;
-                    if (d > 0.0f) s.add(d, (u - (d - e)) - (v + e));
+                for (int k = 0; k < kAtOnce; k++) {   // as probability(): below infinity's bits, which every negative is above
+                    a[k] = __float_as_uint(a[k]) < 0x7f800000u ? a[k] : 0.0f;
+                    b[k] = __float_as_uint(b[k]) < 0x7f800000u ? b[k] : 0.0f;
+                }
+                if (!draft) {
+#pragma unroll
+                    for (int k = 0; k < kAtOnce; k++) s.add(a[k], 0.0f);
+                } else {
+#pragma unroll
+                    for (int k = 0; k < kAtOnce; k++) {
+                        const float d = a[k] - b[k], e = d - a[k];
+                        if (d > 0.0f) s.add(d, (a[k] - (d - e)) - (b[k] + e));
+                    }
                 }
             }
             sum = (double)s.hi + (double)s.lo;
@@ -196,47 +201,83 @@ __global__ void __launch_bounds__(kThreads) tree_verify(VerifyParams p) {
     // The walk, the same in every thread. An accepted child lies behind its parent and its siblings are tried in order, so
     // one run over the nodes meets them all.
     int count = 1, tried = 0;
-    bool counted = false;     // `whole` is the sum of what is left now
     int known = -1;           // rejections that the sums of the last pass have in them
+    bool apart = false;       // without draft rows: the last pass left out the tokens of all children, and
+    double others = 0.0;      // this is its sum
+    bool plain = p.draft;     // a rejection is a pass
     double whole = 1.0;       // what r is divided by
-    double least = 0.0;       // down to what `whole` may be taken less without another pass
     if (rank == 0 && tid == 0) p.path[first] = 0;
     for (int i = 1; i < t.live; i++) {
         if (s_parent[i] != here) continue;
         const int x = s_token[i];
         const double q = p.draft ? probability(s_q[i]) : 1.0;
-        const double r = left_of(probability(s_p[i]), q, x, tried);
+        const double r = apart ? (double)s_c[i] : left_of(probability(s_p[i]), q, x, tried);
         if ((double)s_u[i] * q * whole < r) {
             here = i;
             if (rank == 0 && tid == 0) p.path[first + count] = i;
             count++;
             tried = 0;
             whole = 1.0;
-            counted = false;
+            apart = false;
+            plain = p.draft;
             known = -1;
             continue;
         }
         __syncthreads();
+        if (!plain && !apart) {
+            // the children, in order: their tokens, their own part of the mass, that of those behind them
+            const bool child = tid < t.live && s_parent[tid] == here;
+            const int kids = __syncthreads_count(child);
+            if (child) {
+                int before = 0;
+                bool again = false;
+                for (int k = here + 1; k < tid; k++) {
+                    if (s_parent[k] != here) continue;
+                    before++;
+                    again = again || s_token[k] == s_token[tid];
+                }
+                s_left.token[before] = s_token[tid];
+                s_c[tid] = again ? 0.0f : (float)probability(s_p[tid]);
+            }
+            __syncthreads();
+            if (child) {
+                double after = 0.0;
+                for (int k = t.live - 1; k > tid; k--)
+                    if (s_parent[k] == here) after += (double)s_c[k];
+                s_after[tid] = after;
+            }
+            others = pass(kids);
+            apart = true;
+            known = tried = kids;
+        }
+        if (apart) {
+            const double sum = others + s_after[i];
+            if (sum > 0.0) {
+                whole = sum;
+                continue;
+            }
+            // Nothing would be left: r stays what it was before this child, the mass of this child's token alone. (From here on
+            // as with draft rows.)
+            apart = false;
+            plain = true;
+            known = -1;
+            tried = 0;
+            for (int k = here + 1; k < i; k++) tried += s_parent[k] == here;
+            continue;
+        }
         if (tid == 0) {
             s_left.token[tried] = x;
             if (tried > 0) s_left.inverse[tried - 1] = 1.0 / whole;
         }
         __syncthreads();
-        double sum;
-        if (!p.draft && counted && whole - r >= least) {
-            sum = whole - r;   // (r is 0 if the token has left before)
-        } else {
-            sum = pass(tried + 1, known);
-            known = sum > 0.0 ? tried + 1 : -1;
-            least = sum * 0x1p-10;   // (the rounding of what is taken away stays 2^-43 of what is left)
-        }
+        const double sum = pass(tried + 1);
+        known = sum > 0.0 ? tried + 1 : -1;
         if (sum > 0.0) {
             tried++;
             whole = sum;
-            counted = true;
         }
     }
-    if (known != tried) whole = pass(tried, known);
+    if (known != tried) whole = pass(tried);
     if (rank == 0) {
         for (int i = count + tid; i < p.nodes; i += kThreads) p.path[first + i] = -1;
         if (tid == 0) p.count[slot] = count;
@@ -326,11 +367,11 @@ __global__ void __launch_bounds__(kThreads) tree_verify(VerifyParams p) {
 
 namespace {
 
-// Whether the current device runs a cluster of sixteen CTAs of the kernel.
-bool sixteen_together() {
+// How many clusters of sixteen CTAs of the kernel the current device runs at a time.
+int sixteen_together() {
     if (cudaFuncSetAttribute(tree_verify<16>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess) {
         cudaGetLastError();
-        return false;
+        return 0;
     }
     cudaLaunchAttribute size = {};
     size.id = cudaLaunchAttributeClusterDimension;
@@ -344,9 +385,9 @@ bool sixteen_together() {
     int clusters = 0;
     if (cudaOccupancyMaxActiveClusters(&clusters, tree_verify<16>, &config) != cudaSuccess) {
         cudaGetLastError();
-        return false;
+        return 0;
     }
-    return clusters > 0;
+    return clusters;
 }
 
 }  // namespace
@@ -357,18 +398,16 @@ bool sixteen_together() {
 // 8 slots of 16 nodes of 50,257 with draft rows 17.5 (several rejections in a row, a pass each), 32 slots of 8 nodes of
 // 151,936 without draft rows 32, of which the bytes take 3: the slots are not all there at once.
 int launch_tree_verify(cudaStream_t stream, const VerifyParams &p) {
-    if (p.slots * 16 <= device_sms()) {
-        static std::atomic<int> sixteen[64];   // 0: not asked yet, 1: works, 2: does not
-        int dev = 0;
-        cudaGetDevice(&dev);
-        const bool known = dev >= 0 && dev < 64;
-        int works = known ? sixteen[dev].load() : 0;
-        if (works == 0) {
-            works = sixteen_together() ? 1 : 2;
-            if (known) sixteen[dev].store(works);
-        }
-        if (works == 1) return launch_pdl(tree_verify<16>, dim3(p.slots * 16), dim3(kThreads), 0, stream, 16, p);
+    static std::atomic<int> sixteen[64];   // one more than clusters; 0: not asked yet
+    int dev = 0;
+    cudaGetDevice(&dev);
+    const bool known = dev >= 0 && dev < 64;
+    int most = known ? sixteen[dev].load() : 0;
+    if (most == 0) {
+        most = sixteen_together() + 1;
+        if (known) sixteen[dev].store(most);
     }
+    if (p.slots < most) return launch_pdl(tree_verify<16>, dim3(p.slots * 16), dim3(kThreads), 0, stream, 16, p);
     return launch_pdl(tree_verify<8>, dim3(p.slots * 8), dim3(kThreads), 0, stream, 8, p);
 }
 

@@ -581,6 +581,22 @@ def test_rejected_tokens_that_hold_nearly_all():
         _, count, _ = _verify([R.star(nodes)], tokens, target, None, u, [nodes])
 
 
+def test_looked_up_children_that_hold_all_of_the_mass():
+    """Rejections without draft rows down to nothing: the last token with mass stays, for later siblings and the next token."""
+    nodes, vocab = 8, 200
+    for mass, tokens in (([(5, 0.5), (9, 0.5)], [0, 5, 9, 7, 9, 5, 9, 3]), ([(5, 1.0)], [0, 5, 7, 5, 8, 5, 5, 5]),
+                         ([(5, 1.0)], [0, 7, 8, 5, 5, 7, 5, 9]), ([], [0, 5, 7, 5, 8, 5, 5, 5]),
+                         ([(5, 0.25), (9, 0.5), (199, 0.25)], [0, 9, 9, 199, 9, 5, 5, 9])):
+        target = np.zeros((1, nodes, vocab), dtype=np.float32)
+        for x, m in mass:
+            target[0, :, x] = m
+        # (no random number of 1: a first token that has all of the mass is kept; larger ones make the walk refuse it)
+        for u in (0.5, 0.99, 1.0, 4.0):
+            for parents in (R.star(nodes), [-1, 0, 0, 0, 3, 3, 0, 6]):
+                for u0 in (0.0, 0.6):
+                    _verify([parents], [tokens], target, None, np.array([[u0] + [u] * (nodes - 1)], dtype=np.float32), [nodes])
+
+
 def test_siblings_with_the_same_token():
     rng = np.random.default_rng(12)
     for _ in range(6):
