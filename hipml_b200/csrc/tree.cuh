@@ -29,7 +29,7 @@ struct TreeParams {
     float scale_log2;
     size_t slot_bytes;
     int grid, tile_rows;
-    unsigned group_inverse;   // 65536 / group, rounded up
+    unsigned group_inverse;   // 65536 / group, rounded up: exact for groups of at most 8 and the rows of 256 nodes
     // row / group, of the rows of a slot (fewer than 65536 / 8)
     __device__ __forceinline__ int node_of(int row) const { return (int)((unsigned)row * group_inverse >> 16); }
 };

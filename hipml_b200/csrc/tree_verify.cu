@@ -58,7 +58,7 @@ struct LongSum {
 
 // grid slots * kCtas, clusters of kCtas.
 template <int kCtas>
-__global__ void __launch_bounds__(kThreads) tree_verify(VerifyParams p) {
+__global__ void __launch_bounds__(kThreads, 2) tree_verify(VerifyParams p) {
     __shared__ int s_parent[kTreeNodes], s_token[kTreeNodes];
     __shared__ float s_u[kTreeNodes], s_p[kTreeNodes], s_q[kTreeNodes];
     __shared__ Left s_left;
@@ -123,8 +123,8 @@ __global__ void __launch_bounds__(kThreads) tree_verify(VerifyParams p) {
         const int w0 = min(v0 + warp * run, v1), w1 = min(w0 + run, v1);
         // Most often what is left is p or max(p - q, 0): in f32 with the rounding error beside it, which is as exact here and
         // an eighth of the instructions in 64 bits. (The loops are loops: this code runs once or twice a launch, and its
-        // lines come from beyond the instruction cache: unrolled in 64 bits 8 nodes of 151,936 took 30 us, so 12. Sixteen
-        // values at once take 80 registers, which leaves an SM one CTA: 32 slots of 8 nodes 62 us, with eight 32.)
+        // lines come from beyond the instruction cache: unrolled in 64 bits 8 nodes of 151,936 took 30 us, so 10. Sixteen
+        // values at once take 80 registers, which leaves an SM one CTA: 32 slots of 8 nodes 62 us, with eight 33.)
         double sum = 0.0;
         if (!p.draft || tried <= 1) {
             LongSum s;
@@ -392,11 +392,12 @@ int sixteen_together() {
 
 }  // namespace
 
-// Few slots take clusters of sixteen, which is more than every device must have and is asked for once; many fill it by eights.
+// Clusters of sixteen, which is more than every device must have and is asked for once, as long as all of them fit; more slots
+// take eights (10 slots of 8 nodes of 151,936 with draft rows: 37 us, with eights 60).
 // What bounds it is latency, not memory: a trip for the tree, one for what the walk asks, one pass, the exchange of its sums
-// and the segment of the drawn token follow one another. 8 nodes of 151,936 take 11.6 us (16 slots' rows would pass in 3),
-// 8 slots of 16 nodes of 50,257 with draft rows 17.5 (several rejections in a row, a pass each), 32 slots of 8 nodes of
-// 151,936 without draft rows 32, of which the bytes take 3: the slots are not all there at once.
+// and the segment of the drawn token follow one another. 8 nodes of 151,936 take 9.9 us, 8 slots of 16 nodes of 50,257 with
+// draft rows 17.5 (several rejections in a row, a pass each), 32 slots of 8 nodes of 151,936 without draft rows 18 (their rows
+// pass in 3).
 int launch_tree_verify(cudaStream_t stream, const VerifyParams &p) {
     static std::atomic<int> sixteen[64];   // one more than clusters; 0: not asked yet
     int dev = 0;
