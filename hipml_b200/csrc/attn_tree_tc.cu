@@ -24,9 +24,10 @@
 // Where the time goes (a quantised tile of 64 rows): the MMAs 3,330 cycles (48 of N = 64, 32 cycles with A from TMEM and 48
 // with A from shared memory, and 24 of N = 128, 64 cycles); shared memory as much: the raw bytes in and out (1.1 KB a row),
 // the planes (2), K and the low part of Q into the pipe (2.5), V (1.5), 55 cycles a row. So Q's high part and W come from
-// TMEM: Q hi takes 128 of the 512 columns, O 256, two S tiles 128. A tile takes 5,400 to 6,000 cycles, 64 nodes of eight
-// heads over 100,000 rows 480 us (of a run under the power cap 530): both products and the planes share the issue slots of
-// 20 warps. One warp group more for the planes (24 warps) changed nothing, nor did a third stage of V.
+// TMEM: Q hi takes 128 of the 512 columns, O 256, two S tiles 128. A tile takes 5,500 to 6,000 cycles, 64 nodes of 24 heads
+// (four KV heads) over 100,000 rows 490 us (in a run under the power cap 550): the tensor pipe is 44 % busy and the issue
+// slots 47 %, and the planes, Q K^T, the softmax and W V wait for one another. Four more warps for the planes changed
+// nothing, nor did a third stage of V.
 // Short calls are bound by what comes before the first tile: the launch, the tree, Q's planes, one trip to memory after
 // another and the code's own lines (the loops are loops for that reason).
 //
