@@ -1,0 +1,47 @@
+"""Tree speculation at its edges: rows that are not finite, operators in a row, sums that nearly tie, lengths at the ends of
+their types."""
+import numpy as np
+import pytest
+import torch
+
+from hipml_b200 import api
+from tests import tree_reference as R
+from tests.test_gpu_tree import Step, _dev, _ints, _spoil, status  # noqa: F401 (status: every test leaves the device's clear)
+
+pytestmark = pytest.mark.gpu
+
+
+# ---- attention ---------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("dim", [64, 256])
+@pytest.mark.parametrize("kv_dtype", [0, 1, 2], ids=["f32", "q8", "q4"])
+@pytest.mark.parametrize("value", [float("nan"), float("inf")])
+@pytest.mark.parametrize("which", [(0,), (1,), (0, 1)], ids=["k", "v", "kv"])
+def test_a_run_of_rows_that_are_not_finite(dim, kv_dtype, value, which):
+    """Of two roots behind 128 rows one's own row is all that it sees of the last run; where that is not finite, neither is
+    the node. The other root does not see it."""
+    step = Step(1, kv_dtype, [(128, 2, [-1, -1])], 2, heads=4, kv=2, dim=dim)
+    for w in which:
+        _spoil(step, w, 0, 128, value)
+    step.upload()
+    step.call()
+    got = step.out.cpu().numpy().reshape(2, 4, dim)
+    want, bound = R.attention(step.caches, 0, 128, 2, [-1, -1], step.q[0].reshape(2, 4, dim), 4, step.scale)
+    assert not np.isfinite(got[0]).any()
+    assert (np.abs(got[1] - want[1]) <= bound[1]).all()
+
+
+@pytest.mark.parametrize("dim", [64, 256])
+@pytest.mark.parametrize("kv_dtype", [0, 1, 2], ids=["f32", "q8", "q4"])
+@pytest.mark.parametrize("which", [0, 1], ids=["k", "v"])
+def test_a_whole_tile_of_rows_that_are_not_finite(dim, kv_dtype, which):
+    """64 rows of the prefix of one of two slots; of many runs exactly one has nothing else."""
+    step = Step(2, kv_dtype, [(512, 3, R.chain(3)), (300, 2, R.chain(2))], 3, heads=4, kv=2, dim=dim)
+    for row in range(128, 192):
+        _spoil(step, which, 0, row, float("nan"))
+    step.upload()
+    step.call()
+    got = step.out.cpu().numpy().reshape(2, 3, 4, dim)
+    assert not np.isfinite(got[0]).any()
+    want, bound = R.attention(step.caches, 1, 300, 2, R.chain(2), step.q[1].reshape(3, 4, dim), 4, step.scale)
+    assert (np.abs(got[1, :2] - want) <= bound).all()
