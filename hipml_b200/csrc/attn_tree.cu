@@ -128,6 +128,11 @@ __global__ void __launch_bounds__(256) attn_tree_scalar(TreeParams p) {
             bool sees = r < rows && k0 + lane < hi;
             if (sees && drafted >= 0) sees = s_sees[r][drafted >> 5] >> (drafted & 31) & 1;
             seen[a] = __ballot_sync(0xffffffffu, sees);
+            if (sees && s[a] == -INFINITY) {   // rare: a key that is not finite does not leave with a weight of 0
+#pragma unroll 1
+                for (int d = 0; d < kD; d++)
+                    if (!(fabsf(krow[d]) < INFINITY)) s[a] = __int_as_float(0x7fffffff);
+            }
             // (a row that sees nothing of these keeps what it has: -inf - -inf must not be formed)
             const float mine = sees ? s[a] : -INFINITY;
             const float m_new = fmaxf(m[a], warp_max(mine));

@@ -45,3 +45,23 @@ def test_a_whole_tile_of_rows_that_are_not_finite(dim, kv_dtype, which):
     assert not np.isfinite(got[0]).any()
     want, bound = R.attention(step.caches, 1, 300, 2, R.chain(2), step.q[1].reshape(3, 4, dim), 4, step.scale)
     assert (np.abs(got[1, :2] - want) <= bound).all()
+
+
+@pytest.mark.parametrize("dim", [64, 256])
+@pytest.mark.parametrize("kv_dtype", [0, 1, 2], ids=["f32", "q8", "q4"])
+@pytest.mark.parametrize("base", [40, 128])
+def test_keys_whose_scores_would_be_minus_infinity(dim, kv_dtype, base):
+    """Queries of one sign and a key of -infinity: the row does not leave with a weight of 0, the node is not finite."""
+    step = Step(3, kv_dtype, [(base, 2, [-1, -1])], 2, heads=4, kv=2, dim=dim)
+    step.q[:] = np.abs(step.q) + 0.5
+    step.caches.put(0, 0, base, np.ones((2, 1, dim)))
+    _spoil(step, 0, 0, base, -float("inf"))
+    if kv_dtype == 2:   # (its codes count from -8: all of them above 0)
+        codes = step.caches.rows(0, 0)[:, base].reshape(2, -1, R.ROW_BYTES[2])[:, :, 2:]
+        codes[:] = 0xFF
+    step.upload()
+    step.call()
+    got = step.out.cpu().numpy().reshape(2, 4, dim)
+    want, bound = R.attention(step.caches, 0, base, 2, [-1, -1], step.q[0].reshape(2, 4, dim), 4, step.scale)
+    assert not np.isfinite(got[0]).any()
+    assert (np.abs(got[1] - want[1]) <= bound[1]).all()
