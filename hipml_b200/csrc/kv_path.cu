@@ -32,6 +32,7 @@ __global__ void __launch_bounds__(kThreads) kv_path_keep(const __grid_constant__
     }
     const TreeSlot t = tree_slot(p.pos, slot, p.stride, p.nodes);
     const int count = __ldcg(p.count + slot);
+    if (t.live == 0) return;   // an idle slot: verification has left its path and count as they were
     bool bad = count < 0 || count > t.live;
     if (tid < count) {
         bad = bad || node <= before || node < 0 || node >= t.live;

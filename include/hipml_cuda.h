@@ -505,7 +505,8 @@ int hipml_tree_verify(hipml_stream_t stream, const int *pos, const int *parents,
 /* The kept path's cache rows move together behind the prefix: in every cache of `layers` layers row
  * base + path[i] becomes row base + i, i < count (path and count as hipml_tree_verify leaves them; the
  * other rows stay). k_caches and v_caches are HOST arrays of `layers` device pointers, all different.
- * A path must ascend and stay among the live nodes: otherwise the slot is left as it was (device status 42).
+ * A path must ascend and stay among the live nodes: otherwise the slot is left as it was (device status 42). A slot
+ * without live nodes is left as it was whatever its path and count hold, which is what verification leaves there.
  * One launch for up to 64 layers; cache addresses are taken at the call. */
 int hipml_kv_path_keep(hipml_stream_t stream, int kv_dtype, const int *pos, const int *path,
                        const int *count, void *const *k_caches, void *const *v_caches, int layers,

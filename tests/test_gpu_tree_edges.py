@@ -65,3 +65,40 @@ def test_keys_whose_scores_would_be_minus_infinity(dim, kv_dtype, base):
     want, bound = R.attention(step.caches, 0, base, 2, [-1, -1], step.q[0].reshape(2, 4, dim), 4, step.scale)
     assert not np.isfinite(got[0]).any()
     assert (np.abs(got[1] - want[1]) <= bound[1]).all()
+
+
+# ---- the operators in a row --------------------------------------------------------------------------------------
+
+def test_a_slot_that_goes_idle_between_steps():
+    """Verification leaves an idle slot's path and count as the step before left them; the kept path is not theirs to move."""
+    rng = np.random.default_rng(5)
+    nodes, vocab, kv, dim, stride = 5, 20, 2, 64, 40
+    target = torch.zeros(2, nodes, vocab, device="cuda")
+    tokens = np.array([[0, 3, 4, 5, 6]] * 2)
+    parents = [[-1, 0, 0, 2, 3]] * 2
+    target[:, 0, 4] = target[:, 2, 5] = target[:, 3, 1] = 1.0    # path 0, 2, 3
+    path, count, following = (torch.full(s, -7, dtype=torch.int32, device="cuda") for s in ((2, nodes), (2,), (2,)))
+    host = [rng.integers(0, 256, (2, kv, stride, dim // 32 * 34), dtype=np.uint8) for _ in range(2)]
+    caches = [_dev(h) for h in host]
+
+    def step(lives, base):
+        pos = _ints([[b, b + n] for b, n in zip(base, lives)])
+        api.tree_verify(pos, _ints(parents), _ints(tokens.tolist()), target, None, torch.zeros(2, nodes, device="cuda"), path,
+                        count, following, nodes, 2, vocab)
+        api.kv_path_keep(pos, path, count, caches[:1], caches[1:], kv, dim, stride, nodes, 2, kv * stride * (dim // 32 * 34))
+
+    def keep(slot, base):
+        for h in host:
+            h[slot, :, base:base + 3] = h[slot, :, [base, base + 2, base + 3]].swapaxes(0, 1)
+
+    step((5, 5), (10, 4))
+    keep(0, 10), keep(1, 4)
+    step((0, 5), (13, 7))       # slot 0 idles
+    keep(1, 7)
+    step((0, 0), (13, 10))
+    step((4, 0), (13, 10))
+    keep(0, 13)
+    assert api.check_device_status() == 0
+    assert count.tolist() == [3, 3] and path[:, :3].tolist() == [[0, 2, 3]] * 2
+    for h, c in zip(host, caches):
+        assert np.array_equal(h, c.cpu().numpy())
