@@ -119,6 +119,7 @@ SIGNATURES = {
     "hipml_attn_tree_workspace_bytes": (_sz, [_i, _i, _i, _i, _i]),
     "hipml_attn_tree": (_i, [_vp, _i, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _f, _i, _i, _sz, _vp, _sz]),
     "hipml_tree_verify": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, C.c_longlong]),
+    "hipml_tree_verify_within": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, C.c_longlong, _i]),
     "hipml_kv_path_keep": (_i, [_vp, _i, _vp, _vp, _vp, C.POINTER(_vp), C.POINTER(_vp), _i, _i, _i, _i, _i, _i,
                                 _sz]),
     "hipml_check_device_status": (_i, [_vp, C.POINTER(_i)]),

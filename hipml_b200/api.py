@@ -360,13 +360,19 @@ def attn_tree(pos, parents, q, k_cache, v_cache, out, n_heads, n_kv, head_dim, s
 
 
 def tree_verify(pos, parents, tokens, target, draft, uniform, path, count, next_token, nodes, slots, vocab,
-                row_stride=None):
+                row_stride=None, stride=None):
     """Which drafted nodes are kept and the token that follows them, from target and draft probabilities
     [slots][nodes][vocab] (draft None: looked up) and uniform [slots][nodes] (0: the next token's, i: node i's trial).
 
-    Writes path [slots][nodes] (kept nodes, then -1), count [slots] and next_token [slots]."""
-    rc = _c.tree_verify(pos, parents, tokens, target, draft, uniform, path, count, next_token, nodes, slots, vocab,
-                        vocab if row_stride is None else row_stride)
+    Writes path [slots][nodes] (kept nodes, then -1), count [slots] and next_token [slots]. stride: the cache's rows, past
+    which no node is live (None: every slot's nodes lie within the cache)."""
+    row_stride = vocab if row_stride is None else row_stride
+    if stride is None:
+        rc = _c.tree_verify(pos, parents, tokens, target, draft, uniform, path, count, next_token, nodes, slots, vocab,
+                            row_stride)
+    else:
+        rc = _c.tree_verify_within(pos, parents, tokens, target, draft, uniform, path, count, next_token, nodes, slots,
+                                   vocab, row_stride, stride)
     if rc:
         _lib.check("tree_verify", rc)
 

@@ -997,10 +997,10 @@ int hipml_attn_tree(hipml_stream_t stream, int kv_dtype, const int *pos, const i
     return launch_tree_fold(as_stream(stream), p);
 }
 
-int hipml_tree_verify(hipml_stream_t stream, const int *pos, const int *parents, const int *tokens, const float *target,
-                      const float *draft, const float *uniform, int *path, int *count, int *next, int nodes, int slots,
-                      int vocab, long long row_stride) {
-    if (int e = check_tree(0, 1, 32, 1, nodes, slots)) return e;
+int hipml_tree_verify_within(hipml_stream_t stream, const int *pos, const int *parents, const int *tokens,
+                             const float *target, const float *draft, const float *uniform, int *path, int *count,
+                             int *next, int nodes, int slots, int vocab, long long row_stride, int stride) {
+    if (int e = check_tree(0, 1, 32, stride, nodes, slots)) return e;
     if (vocab < 1 || vocab > kVerifyVocab)
         return fail(HIPML_ERR_INVALID_ARGUMENT, "vocabulary of %d tokens: must be 1..=%d", vocab, kVerifyVocab);
     if (row_stride < vocab)
@@ -1008,9 +1008,16 @@ int hipml_tree_verify(hipml_stream_t stream, const int *pos, const int *parents,
     if (!pos || !parents || !tokens || !target || !uniform || !path || !count || !next)
         return fail(HIPML_ERR_INVALID_ARGUMENT, "tree verification: a tensor is missing");
     VerifyParams p = {pos, parents, tokens, target, draft, uniform, path, count, next, status_of_device(),
-                      nodes, slots, vocab, row_stride};
+                      nodes, slots, vocab, row_stride, stride};
     if (!p.status) return launch_status();
     return launch_tree_verify(as_stream(stream), p);
+}
+
+int hipml_tree_verify(hipml_stream_t stream, const int *pos, const int *parents, const int *tokens, const float *target,
+                      const float *draft, const float *uniform, int *path, int *count, int *next, int nodes, int slots,
+                      int vocab, long long row_stride) {
+    return hipml_tree_verify_within(stream, pos, parents, tokens, target, draft, uniform, path, count, next, nodes, slots,
+                                    vocab, row_stride, 0x7fffffff);
 }
 
 int hipml_kv_path_keep(hipml_stream_t stream, int kv_dtype, const int *pos, const int *path, const int *count,

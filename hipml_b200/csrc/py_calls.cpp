@@ -224,6 +224,7 @@ PyMethodDef kMethods[] = {
     CALL("attn_front_append_q8", front_append),
     CALL("attn_tree", hipml_attn_tree),
     CALL("tree_verify", hipml_tree_verify),
+    CALL("tree_verify_within", hipml_tree_verify_within),
     CALL("kv_path_keep", path_keep),
     {nullptr, nullptr, 0, nullptr},
 };

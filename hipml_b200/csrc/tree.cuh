@@ -200,6 +200,7 @@ struct VerifyParams {
     int *status;
     int nodes, slots, vocab;
     long long row_stride;
+    int stride;            // rows of the cache that the nodes' rows lie in
 };
 int launch_tree_verify(cudaStream_t stream, const VerifyParams &p);
 

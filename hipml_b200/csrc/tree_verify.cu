@@ -82,7 +82,7 @@ __global__ void __launch_bounds__(kThreads, 2) tree_verify(VerifyParams p) {
         x_of = tid == 0 ? 0 : __ldcg(p.tokens + first + tid);
         s_u[tid] = __ldcg(p.uniform + first + tid);
     }
-    const TreeSlot t = tree_slot(p.pos, slot, 0x7fffffff, p.nodes);
+    const TreeSlot t = tree_slot(p.pos, slot, p.stride, p.nodes);
     if (t.live == 0) return;   // (the whole cluster) nothing is written
     if (tid < t.live) {
         if (up >= tid || up < -1 || x_of < 0 || x_of >= p.vocab) {

@@ -86,6 +86,7 @@ extern "C" {
     pub fn hipml_attn_tree_workspace_bytes(n_heads: c_int, n_kv: c_int, head_dim: c_int, nodes: c_int, slots: c_int) -> usize;
     pub fn hipml_attn_tree(stream: Stream, kv_dtype: c_int, pos: *const c_int, parents: *const c_int, q: *const f32, k_cache: *const c_void, v_cache: *const c_void, out: *mut f32, n_heads: c_int, n_kv: c_int, head_dim: c_int, stride: c_int, scale: f32, nodes: c_int, slots: c_int, kv_slot_bytes: usize, workspace: *mut c_void, workspace_bytes: usize) -> Status;
     pub fn hipml_tree_verify(stream: Stream, pos: *const c_int, parents: *const c_int, tokens: *const c_int, target: *const f32, draft: *const f32, uniform: *const f32, path: *mut c_int, count: *mut c_int, next: *mut c_int, nodes: c_int, slots: c_int, vocab: c_int, row_stride: i64) -> Status;
+    pub fn hipml_tree_verify_within(stream: Stream, pos: *const c_int, parents: *const c_int, tokens: *const c_int, target: *const f32, draft: *const f32, uniform: *const f32, path: *mut c_int, count: *mut c_int, next: *mut c_int, nodes: c_int, slots: c_int, vocab: c_int, row_stride: i64, stride: c_int) -> Status;
     pub fn hipml_kv_path_keep(stream: Stream, kv_dtype: c_int, pos: *const c_int, path: *const c_int, count: *const c_int, k_caches: *const *mut c_void, v_caches: *const *mut c_void, layers: c_int, n_kv: c_int, head_dim: c_int, stride: c_int, nodes: c_int, slots: c_int, kv_slot_bytes: usize) -> Status;
     pub fn hipml_set_decode_cta_slots(slots: c_int) -> Status;
     pub fn hipml_set_decode_body(body: c_int) -> Status;

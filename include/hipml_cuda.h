@@ -464,9 +464,10 @@ int hipml_attn_chunk_staged_gated(hipml_stream_t stream, const float *q, float *
  * cache row base + i (append them with hipml_kv_encode_bulk, hipml_kv_append_cols_f32 or
  * hipml_attn_front_append_q8). parents is device i32 [slots][nodes]: the parent of node i, an
  * earlier node (< i), or -1. Nothing of a node past a slot's live ones is used or written, whatever
- * the buffers hold there; lengths past the cache count as the cache. kv_dtype, caches and stride
- * are those of hipml_attn_chunk (0 f32 [stride][n_kv*head_dim], 1 q8_0, 2 q4_0 head-major), slot s
- * begins at byte s*kv_slot_bytes (any value where slots is 1). 1..65535 slots. A parent that is no
+ * the buffers hold there; lengths past the cache count as the cache (hipml_tree_verify knows none:
+ * hipml_tree_verify_within). kv_dtype, caches and stride are those of hipml_attn_chunk (0 f32
+ * [stride][n_kv*head_dim], 1 q8_0, 2 q4_0 head-major), slot s begins at byte
+ * s*kv_slot_bytes (any value where slots is 1). 1..65535 slots. A parent that is no
  * earlier node ends that node's ancestors there and is reported by hipml_check_device_status as 41.
  * All of it can be captured and replayed: lengths, trees and paths are read on the device. Calls that may
  * overlap on the device must not share a workspace; nothing else is shared between calls.
@@ -501,6 +502,13 @@ int hipml_attn_tree(hipml_stream_t stream, int kv_dtype, const int *pos, const i
 int hipml_tree_verify(hipml_stream_t stream, const int *pos, const int *parents, const int *tokens,
                       const float *target, const float *draft, const float *uniform, int *path,
                       int *count, int *next, int nodes, int slots, int vocab, long long row_stride);
+/* The same over the nodes that a cache of `stride` rows holds: those of a tree that crosses its end which attention and
+ * the kept path leave out are not kept, and nothing of their rows is read. hipml_tree_verify knows no cache: there
+ * base + live nodes has to lie within it. */
+int hipml_tree_verify_within(hipml_stream_t stream, const int *pos, const int *parents, const int *tokens,
+                             const float *target, const float *draft, const float *uniform, int *path,
+                             int *count, int *next, int nodes, int slots, int vocab, long long row_stride,
+                             int stride);
 
 /* The kept path's cache rows move together behind the prefix: in every cache of `layers` layers row
  * base + path[i] becomes row base + i, i < count (path and count as hipml_tree_verify leaves them; the

@@ -102,3 +102,30 @@ def test_a_slot_that_goes_idle_between_steps():
     assert count.tolist() == [3, 3] and path[:, :3].tolist() == [[0, 2, 3]] * 2
     for h, c in zip(host, caches):
         assert np.array_equal(h, c.cpu().numpy())
+
+
+@pytest.mark.parametrize("looked_up", [False, True], ids=["drawn", "looked up"])
+def test_trees_that_cross_the_end_of_the_cache(looked_up):
+    """Attention, verification and the kept path agree on which nodes the cache has: the last two are not among them, although
+    their tokens would be kept (their target rows hold what nobody computed)."""
+    nodes, vocab, kv, dim, stride, base = 6, 30, 2, 64, 50, 46
+    parents = R.chain(nodes)
+    step = Step(7, 1, [(base, 4, parents)], nodes, heads=4, kv=kv, dim=dim, stride=stride)
+    step.parents[:] = parents
+    step.dparents, step.pos = _dev(step.parents), _ints([[base, base + nodes]])
+    step.run()
+    tokens = [0, 1, 2, 3, 4, 5]
+    target = np.full((1, nodes, vocab), np.nan, dtype=np.float32)
+    target[0, :4] = 0.5 / vocab
+    for i in range(4):
+        target[0, i, i + 1] = 0.5
+    draft = None if looked_up else np.full((1, nodes, vocab), 1.0 / vocab, dtype=np.float32)
+    u = np.full((1, nodes), 0.25, dtype=np.float32)
+    path, count, following = (torch.full(s, -7, dtype=torch.int32, device="cuda") for s in ((1, nodes), (1,), (1,)))
+    api.tree_verify(step.pos, step.dparents, _ints([tokens]), _dev(target), None if looked_up else _dev(draft), _dev(u), path,
+                    count, following, nodes, 1, vocab, stride=stride)
+    want, token = R.verify(parents, tokens, target[0], None if looked_up else draft[0], u[0], 4)
+    assert want == [0, 1, 2, 3]
+    assert path[0].tolist() == want + [-1, -1] and count.tolist() == [4] and following.tolist() == [token]
+    api.kv_path_keep(step.pos, path, count, [step.dk], [step.dv], kv, dim, stride, nodes, 1, 0)
+    assert api.check_device_status() == 0

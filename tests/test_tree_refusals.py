@@ -170,3 +170,11 @@ def test_the_rule_emits_the_targets_distribution():
                             got[R.verify(R.star(3), [0, a, b], target, draft, [u0, u1, u2], 3)[1]] += w / n
     # each of the three numbers moves a share of at most one cell of the grid
     assert np.abs(got - p).max() <= 3.0 / n
+
+
+@pytest.mark.parametrize("stride", [0, -5])
+def test_verification_refuses_a_cache_without_rows(stride):
+    with pytest.raises(_lib.HipmlError, match=f"stride {stride} must be positive"):
+        api.tree_verify(T, T, T, T, None, T, T, T, T, 8, 1, 100, stride=stride)
+    with pytest.raises(_lib.HipmlError, match="vocabulary of 0"):   # the bound changes nothing of the other refusals
+        api.tree_verify(T, T, T, T, None, T, T, T, T, 8, 1, 0, stride=100)
