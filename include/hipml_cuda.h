@@ -496,7 +496,7 @@ int hipml_attn_tree(hipml_stream_t stream, int kv_dtype, const int *pos, const i
  * no child is kept, `next` is the lowest token whose running sum of r exceeds uniform[0] times
  * the whole (the last token with r > 0 where rounding leaves none; -1 where r has no mass). path i32
  * [slots][nodes] receives the kept nodes in order, then -1; count i32 [slots] how many. Outputs of a
- * slot without live nodes stay as they are. Sums are exact to 2^-45. What is no probability (NaN,
+ * slot without live nodes stay as they are. Sums are exact to 2^-43. What is no probability (NaN,
  * negative, infinite) counts as 0; a child whose parent is no earlier node or whose token is not in
  * the vocabulary is never kept (device status 41). vocab 1..1048576. */
 int hipml_tree_verify(hipml_stream_t stream, const int *pos, const int *parents, const int *tokens,

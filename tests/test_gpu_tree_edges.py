@@ -129,3 +129,45 @@ def test_trees_that_cross_the_end_of_the_cache(looked_up):
     assert path[0].tolist() == want + [-1, -1] and count.tolist() == [4] and following.tolist() == [token]
     api.kv_path_keep(step.pos, path, count, [step.dk], [step.dv], kv, dim, stride, nodes, 1, 0)
     assert api.check_device_status() == 0
+
+
+# ---- sums --------------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("rejected", [False, True], ids=["root", "rejected"])
+@pytest.mark.parametrize("drawn", [False, True], ids=["looked up", "drawn"])
+@pytest.mark.parametrize("short", [False, True], ids=["past", "short"])
+def test_the_longest_rows_where_the_bar_lies_next_to_a_running_sum(rejected, drawn, short):
+    """2^20 tokens, whole numbers of 2^-61 whose running sum over the first half is 2^-43 of the whole past half of the whole,
+    or short of it. The first 32 values of every 4,096 are large and the rest lie 2^-25 below them, in the second half by a
+    little less, which a long running error in 32 bits loses each time.
+
+    Sums are exact to less than 2^-43 of what is summed: the bar (half of the whole) and the running sum (as much) together
+    are less than 2^-43 of the whole off."""
+    vocab, half, gone = 1 << 20, 1 << 19, (1 << 19) + 100
+    units = np.full(vocab, 1 << 23, dtype=np.int64)
+    units[half:] += 31
+    units.reshape(-1, 4096)[:, :32] = 1 << 48
+    units[gone] = 0   # the rejected child's token
+    off = int(units.sum()) >> 43
+    over = int(units[half:].sum()) - int(units[:half].sum()) - (2 * off if short else -2 * off)
+    for at in range(vocab - 1, half, -1):   # the last tokens give what the second half has too much
+        less = min(over, int(units[at]))
+        units[at] -= less
+        over -= less
+        if over == 0:
+            break
+    row = (units * 2.0 ** -61).astype(np.float32)
+    assert over == 0 and np.array_equal(row.astype(np.float64) * 2.0 ** 61, units)
+    whole, front = int(units.sum()), int(units[:half].sum())
+    assert (2 * front > whole) == (not short) and whole >> 44 <= abs(2 * front - whole) // 2 <= whole >> 42
+    want = half if short else half - 1
+    target = _dev(np.stack([row, row])[None])
+    draft = None
+    if drawn:
+        draft = torch.zeros(1, 2, vocab, device="cuda")
+        draft[0, 0, gone] = 1.0
+    path, count, following = (torch.full(s, -7, dtype=torch.int32, device="cuda") for s in ((1, 2), (1,), (1,)))
+    api.tree_verify(_ints([[3, 5 if rejected else 4]]), _ints([[-1, 0]]), _ints([[0, gone]]), target, draft,
+                    torch.full((1, 2), 0.5, device="cuda"), path, count, following, 2, 1, vocab)
+    assert count.tolist() == [1] and path.tolist() == [[0, -1]]
+    assert following.tolist() == [want]
