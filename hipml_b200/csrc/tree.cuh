@@ -55,7 +55,7 @@ __device__ __forceinline__ TreeSlot tree_slot(const int *pos, int slot, int stri
     const int from = __ldcg(pos + 2 * (size_t)slot), to = __ldcg(pos + 2 * (size_t)slot + 1);
     TreeSlot s;
     s.base = min(max(from, 0), stride);
-    s.live = min(max(min(to, stride) - s.base, 0), nodes);
+    s.live = min(max(min(max(to, 0), stride) - s.base, 0), nodes);   // (of numbers that are not negative: no difference wraps)
     return s;
 }
 

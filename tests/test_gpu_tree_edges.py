@@ -67,6 +67,25 @@ def test_keys_whose_scores_would_be_minus_infinity(dim, kv_dtype, base):
     assert (np.abs(got[1] - want[1]) <= bound[1]).all()
 
 
+def test_ends_at_the_edge_of_their_type():
+    """The end words of pos are any 32-bit numbers: a negative end is an empty slot, an end past the cache the cache's."""
+    low, high = -(1 << 31), (1 << 31) - 1
+    tree = R.chain(4)
+    for dim in (64, 256):
+        step = Step(4, 1, [(70, 0, tree), (1, 0, tree), (60, 4, tree), (0, 4, tree), (70, 0, tree)], 4, heads=4, kv=2, dim=dim,
+                    stride=70)
+        step.parents[:] = tree
+        step.dparents = _dev(step.parents)
+        step.pos = _ints([[70, low], [1, low], [60, 64], [low, 4], [high, low]])
+        step.run()
+        step.pos = _ints([[70, high], [1, low + 5], [60, 64], [low, 4], [high, high]])
+        step.run()
+    path, count, following = (torch.full((n,), 9, dtype=torch.int32, device="cuda") for n in (12, 3, 3))
+    api.tree_verify(_ints([[5, low], [high, low], [1, low + 3]]), _ints([tree] * 3), _ints([[0, 1, 2, 3]] * 3),
+                    torch.ones(3, 4, 5, device="cuda"), None, torch.zeros(3, 4, device="cuda"), path, count, following, 4, 3, 5)
+    assert (torch.cat([path, count, following]) == 9).all()
+
+
 # ---- the operators in a row --------------------------------------------------------------------------------------
 
 def test_a_slot_that_goes_idle_between_steps():
