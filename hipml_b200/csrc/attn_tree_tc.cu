@@ -281,8 +281,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tree_tc(TreeParams p) {
     const TreeItem it = s_item;
     const Waits wait = {&s_abort, p.status};
     const int rows = min(kRows, it.live * p.group - it.tile * kRows);
-    const int len = it.base + it.live;
-    const int lo_key = it.run * it.quota * kTreeKeyTile, hi_key = min(lo_key + it.quota * kTreeKeyTile, len);
+    const int lo_key = it.first_row(), hi_key = it.end_row();
     const int n = it.slot < 0 ? 0 : (hi_key - lo_key + T::kKeys - 1) / T::kKeys;   // tiles
     const size_t first_node = (size_t)it.slot * p.nodes;
     auto head_row = [&](int r) {   // row r of the tile as a row of q and out, in heads

@@ -63,6 +63,12 @@ __device__ __forceinline__ TreeSlot tree_slot(const int *pos, int slot, int stri
 struct TreeItem {
     int slot, kvh, tile, run, runs;
     int base, live, quota;
+    // the run's rows; nothing beyond the slot's last is formed, which may be the largest int
+    __device__ __forceinline__ int first_row() const { return run * quota * kTreeKeyTile; }
+    __device__ __forceinline__ int end_row() const {
+        const int first = first_row(), rows = base + live - first;
+        return first + (int)min((unsigned)quota * kTreeKeyTile, (unsigned)rows);
+    }
 };
 
 // The slots as a warp's lanes hold them: the first 32 stay in registers, so that the plan is one trip to memory.
@@ -79,7 +85,7 @@ struct TreeSlots {
         return s < 32 ? mine : tree_slot(p.pos, s, p.stride, p.nodes);
     }
     static __device__ __forceinline__ unsigned keys(const TreeSlot &t) {   // key tiles
-        return (unsigned)(t.base + t.live + kTreeKeyTile - 1) / kTreeKeyTile;
+        return ((unsigned)(t.base + t.live) + kTreeKeyTile - 1) / kTreeKeyTile;
     }
     __device__ __forceinline__ unsigned tiles(const TreeSlot &t) const {   // of rows
         return (unsigned)(t.live * p.group + kRows - 1) / kRows;
@@ -110,7 +116,7 @@ __device__ __forceinline__ int tree_quota(const TreeParams &p, const TreeSlots<k
             if (runs <= fit) return 1;
             lo = (runs + fit - 1) / fit;
             // sum(rows * ceil(keys / q)) <= runs / q + rows; with one run each, every triple has its CTA
-            hi = fit > rows ? (runs + fit - rows - 1) / (fit - rows) : (unsigned)(p.stride + kTreeKeyTile - 1) / kTreeKeyTile;
+            hi = fit > rows ? (runs + fit - rows - 1) / (fit - rows) : ((unsigned)p.stride + kTreeKeyTile - 1) / kTreeKeyTile;
             q = lo;
             lo--;       // (does not fit; hi does)
             if (hi <= q) return (int)q;

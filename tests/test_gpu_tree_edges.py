@@ -86,6 +86,28 @@ def test_ends_at_the_edge_of_their_type():
     assert (torch.cat([path, count, following]) == 9).all()
 
 
+def test_a_cache_of_as_many_rows_as_an_int_counts():
+    """2^31 - 1 rows of 18 bytes; the last run ends within a tile of the largest int. Keys are 0, so every row counts alike."""
+    stride, live, dim = (1 << 31) - 1, 3, 32
+    if torch.cuda.mem_get_info()[0] < 60 << 30:
+        pytest.skip("needs 39 GB")
+    cache = torch.zeros(stride, 18, dtype=torch.uint8, device="cuda")
+    base = stride - live
+    row = torch.from_numpy(np.frombuffer(np.float16(1.0).tobytes() + bytes([0x9F] * 16), dtype=np.uint8).copy()).cuda()
+    cache[base] = row     # low nibbles 15 (values 7), high ones 9 (values 1)
+    q = torch.zeros(1, live, dim, device="cuda")
+    out = torch.empty(1, live, dim, device="cuda")
+    ws = torch.empty(api.attn_tree_workspace_bytes(1, 1, dim, live, 1), dtype=torch.uint8, device="cuda")
+    api.attn_tree(_ints([[base, stride]]), _ints([[-1, -1, 0]]), q, cache, cache, out, 1, 1, dim, stride, 1.0, live, 1, 0, ws,
+                  kv_dtype=2)
+    got = out.cpu().numpy().reshape(live, dim).astype(np.float64)
+    value = np.r_[np.full(16, 7.0), np.full(16, 1.0)]
+    # (scores are 0: a weight of 1 a row; whole numbers below 2^24 in each of the runs, and then at most 42 sums one after
+    # another, a reciprocal and a product, each rounded by 2^-24 of itself: less than 2^-18)
+    for node, rows, seen in ((0, base + 1, 1), (1, base + 1, 0), (2, base + 2, 1)):
+        assert (np.abs(got[node] - seen * value / rows) <= 2.0 ** -18 * value / rows).all()
+
+
 # ---- the operators in a row --------------------------------------------------------------------------------------
 
 def test_a_slot_that_goes_idle_between_steps():
