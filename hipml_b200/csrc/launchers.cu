@@ -960,6 +960,11 @@ int hipml_attn_tree(hipml_stream_t stream, int kv_dtype, const int *pos, const i
         return fail(HIPML_ERR_INVALID_ARGUMENT, "tree attention: q and out must be 16-byte aligned");
     if (((reinterpret_cast<size_t>(k_cache) | reinterpret_cast<size_t>(v_cache)) & (kv_dtype == 0 ? 3 : 1)) != 0)
         return fail(HIPML_ERR_INVALID_ARGUMENT, "tree attention: the caches must be %d-byte aligned", kv_dtype == 0 ? 4 : 2);
+    // (the plan counts pairs of row tiles and key tiles in 32 bits; fewer fit the device's memory, by far but for rows of 18 bytes)
+    const long long row_tiles = ((long long)nodes * (n_heads / n_kv) + kTreeScalarRows - 1) / kTreeScalarRows;
+    const long long key_tiles = ((long long)stride + kTreeKeyTile - 1) / kTreeKeyTile;
+    if (row_tiles * key_tiles * slots > 0xffffffffLL)
+        return fail(HIPML_ERR_INVALID_ARGUMENT, "tree attention: %d nodes over %d slots of %d rows are too many", nodes, slots, stride);
     const size_t need = hipml_attn_tree_workspace_bytes(n_heads, n_kv, head_dim, nodes, slots);
     if (need == 0) return fail(HIPML_ERR_INVALID_ARGUMENT, "tree attention: %d slots of %d nodes are too many", slots, nodes);
     if (!workspace || workspace_bytes < need)

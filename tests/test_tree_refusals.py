@@ -178,3 +178,16 @@ def test_verification_refuses_a_cache_without_rows(stride):
         api.tree_verify(T, T, T, T, None, T, T, T, T, 8, 1, 100, stride=stride)
     with pytest.raises(_lib.HipmlError, match="vocabulary of 0"):   # the bound changes nothing of the other refusals
         api.tree_verify(T, T, T, T, None, T, T, T, T, 8, 1, 0, stride=100)
+
+
+def test_attention_refuses_more_pairs_of_tiles_than_the_plan_counts():
+    """64 row tiles (256 nodes of eight heads) over 2^25 key tiles are 2^31 pairs: two slots of them do not fit 32 bits."""
+    rows = (1 << 31) - 1
+    with pytest.raises(_lib.HipmlError, match="256 nodes over 2 slots of 2147483647 rows are too many") as e:
+        _attn(heads=8, kv=1, dim=32, nodes=256, slots=2, stride=rows, slot_bytes=rows * 18, kv_dtype=2)
+    assert e.value.code == _lib.ERR_INVALID_ARGUMENT
+    # (one slot, or 128 nodes, are as many as it counts: what is missing there is the workspace)
+    for few in (dict(slots=1), dict(nodes=127)):
+        with pytest.raises(_lib.HipmlError, match="needed"):
+            _attn(**{**dict(heads=8, kv=1, dim=32, nodes=256, slots=2, stride=rows, slot_bytes=rows * 18, kv_dtype=2,
+                            workspace=None), **few})
