@@ -790,21 +790,24 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tree_tc(TreeParams p) {
 #pragma unroll 1
                 for (int j = 0; j < 4; j++) {
                     unsigned v[32];
+                    __syncwarp();
                     tmem_ld32(lane_at + kTmemO + 128 * half + 32 * j, v);
-                    if (!live || *wait.abort) continue;
+                    if (live && !*wait.abort) {
 #pragma unroll
-                    for (int e = 0; e < 32; e += 4) {
-                        const float4 w = make_float4(__uint_as_float(v[e]) * g, __uint_as_float(v[e + 1]) * g,
-                                                     __uint_as_float(v[e + 2]) * g, __uint_as_float(v[e + 3]) * g);
-                        float *const to = flushed + (size_t)(32 * half + 8 * j + e / 4) * (kRows * 4);
-                        if (over)
-                            *reinterpret_cast<float4 *>(to) = w;
-                        else
-                            asm volatile("red.global.add.v4.f32 [%0], {%1, %2, %3, %4};" ::"l"(to), "f"(w.x), "f"(w.y),
-                                         "f"(w.z), "f"(w.w)
-                                         : "memory");
+                        for (int e = 0; e < 32; e += 4) {
+                            const float4 w = make_float4(__uint_as_float(v[e]) * g, __uint_as_float(v[e + 1]) * g,
+                                                         __uint_as_float(v[e + 2]) * g, __uint_as_float(v[e + 3]) * g);
+                            float *const to = flushed + (size_t)(32 * half + 8 * j + e / 4) * (kRows * 4);
+                            if (over)
+                                *reinterpret_cast<float4 *>(to) = w;
+                            else
+                                asm volatile("red.global.add.v4.f32 [%0], {%1, %2, %3, %4};" ::"l"(to), "f"(w.x), "f"(w.y),
+                                             "f"(w.z), "f"(w.w)
+                                             : "memory");
+                        }
                     }
                 }
+                __syncwarp();
                 tc_fence_before();
                 if (over) m_out = m;
             }
@@ -813,6 +816,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tree_tc(TreeParams p) {
                 m = m_new;
             } else if (__any_sync(0xffffffffu, move)) {
                 const float corr = m == -INFINITY ? 0.0f : exp2f(m - m_new);
+                __syncwarp();
 #pragma unroll 1
                 for (int j = 0; j < 4; j++) {
                     unsigned v[32];
@@ -827,6 +831,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tree_tc(TreeParams p) {
             }
             const float shift = value_power - ((m == -INFINITY ? 0.0f : m) - kLift);
             float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+            __syncwarp();
 #pragma unroll
             for (int e0 = 0; e0 < T::kHalf; e0 += 16) {   // per 16 keys: eight words of hi, eight of lo
                 float o[16];
@@ -844,6 +849,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tree_tc(TreeParams p) {
             }
             l = fmaf((sum[0] + sum[1]) + (sum[2] + sum[3]), value_inverse, l);
             if (sum_s != 0.0f) l = fmaf(sum_s, exp2f(most_s - m + kLift), l);
+            __syncwarp();
             tmem_wait_st();
             tc_fence_before();
             __syncwarp();
@@ -866,6 +872,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tree_tc(TreeParams p) {
 #pragma unroll 1
             for (int j = 0; j < 4; j++) {
                 unsigned v[32];
+                __syncwarp();
                 tmem_ld32(lane_at + kTmemO + 128 * half + 32 * j, v);
                 float *const at = staged + r * kOutPitch + dims_of(j);
                 if (join && live) {
