@@ -461,16 +461,23 @@ int hipml_attn_chunk_staged_gated(hipml_stream_t stream, const float *q, float *
  * chains: hipml_attn_decode_cols) ----
  * A slot's tree has up to `nodes` nodes (1..256). pos is device i32 [slots][2] = (base, base + live
  * nodes), the step words of the other entries: the drafted rows lie behind the prefix, node i's in
- * cache row base + i (append them with hipml_kv_encode_bulk, hipml_kv_append_cols_f32 or
- * hipml_attn_front_append_q8). parents is device i32 [slots][nodes]: the parent of node i, an
- * earlier node (< i), or -1. Nothing of a node past a slot's live ones is used or written, whatever
- * the buffers hold there; lengths past the cache count as the cache (hipml_tree_verify knows none:
+ * cache row base + i. Rows are taken as they lie: node i's K row, and its query, must have been rotated
+ * for position base + depth(i), the number of its ancestors, so that siblings have the same position
+ * and a kept row is right where it moves to. What rotates several tokens, each one position on
+ * (hipml_attn_front_append_q8 with tokens > 1, hipml_norm_rope_chunk), is right for chains only; for a
+ * tree that branches call per node hipml_attn_front_append_q8 (q8_0), or hipml_attn_front and then
+ * hipml_kv_encode or hipml_kv_append_f32: pos holds the position ids and step[0] the row base + i,
+ * both read on the device. Rows that are rotated already go into the cache with hipml_kv_encode_bulk
+ * or hipml_kv_append_chunk_f32 (the first row is a host number there, which a capture keeps).
+ *
+ * parents is device i32 [slots][nodes]: the parent of node i, an earlier node (< i), or -1. Nothing of
+ * a node past a slot's live ones is used or written, whatever the buffers hold there; lengths past the cache count as the cache (hipml_tree_verify knows none:
  * hipml_tree_verify_within). kv_dtype, caches and stride are those of hipml_attn_chunk (0 f32
- * [stride][n_kv*head_dim], 1 q8_0, 2 q4_0 head-major), slot s begins at byte
- * s*kv_slot_bytes (any value where slots is 1). 1..65535 slots. A parent that is no
- * earlier node ends that node's ancestors there and is reported by hipml_check_device_status as 41.
- * All of it can be captured and replayed: lengths, trees and paths are read on the device. Calls that may
- * overlap on the device must not share a workspace; nothing else is shared between calls.
+ * [stride][n_kv*head_dim], 1 q8_0, 2 q4_0 head-major), slot s begins at byte s*kv_slot_bytes (any
+ * value where slots is 1). 1..65535 slots. A parent that is no earlier node ends that node's
+ * ancestors there and is reported by hipml_check_device_status as 41. The entries here can be captured
+ * and replayed: lengths, trees and paths are read on the device. Calls that may overlap on the device
+ * must not share a workspace; nothing else is shared between calls.
  *
  * Attention of the drafted nodes in one call: node i sees cache rows [0, base), its own row and
  * those of its ancestors. q and out are f32 [slots][nodes][n_heads*head_dim], 16-byte aligned. A row

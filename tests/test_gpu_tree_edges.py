@@ -212,3 +212,95 @@ def test_the_longest_rows_where_the_bar_lies_next_to_a_running_sum(rejected, dra
                     torch.full((1, 2), 0.5, device="cuda"), path, count, following, 2, 1, vocab)
     assert count.tolist() == [1] and path.tolist() == [[0, -1]]
     assert following.tolist() == [want]
+
+
+# ---- rotated rows ------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("kv_dtype", [0, 1, 2], ids=["f32", "q8", "q4"])
+def test_a_captured_step_of_a_branching_tree_with_rotated_rows(kv_dtype):
+    """Node i's row is rotated for position base + depth(i) and lies at base + i: the front end is called once per node, whose
+    position and row are read on the device. What the step leaves is what the kept tokens as a chain make, byte for byte, for
+    every base and tree that the captured step is replayed with."""
+    heads, kv, dim, n_rot, nodes, stride, vocab = 24, 4, 256, 64, 9, 400, 50
+    theta, eps = 1e6, 1e-6
+    rng = np.random.default_rng(90)
+
+    def floats(*shape):
+        return _dev(rng.standard_normal(shape).astype(np.float32))
+
+    qg, k, v = floats(nodes, heads * 2 * dim), floats(nodes, kv * dim), floats(nodes, kv * dim)
+    qw, kw = floats(dim), floats(dim)
+    q, out = (torch.zeros(1, nodes, heads * dim, device="cuda") for _ in range(2))
+    fresh = R.Caches(kv_dtype, 1, kv, dim, stride, fill=0)
+    caches = [_dev(b) for b in fresh.bytes]
+    ids, steps = torch.zeros(nodes, 4, dtype=torch.int32, device="cuda"), torch.zeros(nodes, 8, dtype=torch.int32, device="cuda")
+    pos, parents = _ints([[0, 0]]), _ints([[-1] * nodes])
+    tokens, uniform = _ints([list(range(nodes))]), torch.zeros(1, nodes, device="cuda")
+    target = torch.zeros(1, nodes, vocab, device="cuda")
+    path, count, following = torch.zeros(1, nodes, dtype=torch.int32, device="cuda"), _ints([0]), _ints([0])
+    ws = torch.empty(api.attn_tree_workspace_bytes(heads, kv, dim, nodes, 1), dtype=torch.uint8, device="cuda")
+
+    def append(pair, token, to_q, at, step):
+        """One token's query and row, at position ids `at` and cache row step[0]."""
+        gate = torch.empty(heads * dim, device="cuda")
+        if kv_dtype == 1:
+            api.attn_front_append_q8(qg[token], k[token], v[token], to_q, gate, qw, kw, *pair, heads, kv, dim, n_rot, theta, eps,
+                                     stride=stride, pos=at, step=step)
+            return
+        row = k[token].clone()   # (rotated in place)
+        api.attn_front(qg[token], to_q, gate, row, qw, kw, heads, kv, dim, n_rot, None, at, theta, eps)
+        if kv_dtype == 2:
+            api.kv_encode(step, row, v[token], *pair, kv, dim, stride, dtype=1)
+        else:
+            api.kv_append_f32(step, pair[0].view(torch.float32), pair[1].view(torch.float32), row, v[token], kv * dim)
+
+    def step():
+        for i in range(nodes):
+            append(caches, i, q[0, i], ids[i], steps[i])
+        api.attn_tree(pos, parents, q, *caches, out, heads, kv, dim, stride, dim ** -0.5, nodes, 1, 0, ws, kv_dtype=kv_dtype)
+        api.tree_verify(pos, parents, tokens, target, None, uniform, path, count, following, nodes, 1, vocab, stride=stride)
+        api.kv_path_keep(pos, path, count, caches[:1], caches[1:], kv, dim, stride, nodes, 1, 0, kv_dtype=kv_dtype)
+
+    stream = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(stream):
+        step()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        step()
+    for base, tree, kept in ((100, [-1, 0, 0, 1, 2, 2, 5, 5, 3], [0, 2, 5, 7]), (391, [-1, 0, 1, 1, 1, 4, 4, 6, 0], [0, 1, 4, 6, 7]),
+                             (0, R.star(nodes), [0, 8])):
+        depth = [len(R.sees(tree, i)) - 1 for i in range(nodes)]
+        ids.copy_(_ints([[base + d] * 4 for d in depth]))
+        steps.copy_(_ints([[base + i] + [0] * 7 for i in range(nodes)]))
+        pos.copy_(_ints([[base, base + nodes]]))
+        parents.copy_(_ints([tree]))
+        target.fill_(0.0)
+        for a, b in zip(kept, kept[1:] + [40]):
+            target[0, a, b] = 1.0   # (node b's token is b)
+        # a prefix; the kept tokens behind it as a chain, and the step over it
+        prefix = R.Caches(kv_dtype, 1, kv, dim, stride, fill=0)
+        if base:
+            prefix.fill(rng, 0, base)
+        chain = [_dev(b) for b in prefix.bytes]
+        for c, b in zip(caches, chain):
+            c.copy_(b)
+        n = len(kept)
+        chain_q = torch.zeros(1, n, heads * dim, device="cuda")
+        for i, token in enumerate(kept):
+            append(chain, token, chain_q[0, i], _ints([base + i] * 4), _ints([base + i] + [0] * 7))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert path[0, :n].tolist() == kept and count.tolist() == [n] and following.tolist() == [40]
+        shape = (stride, kv, dim * 4) if kv_dtype == 0 else (kv, stride, fresh.row)
+        for c, want in zip(caches, chain):
+            c, want = (x.view(torch.uint8).view(shape) for x in (c, want))
+            assert torch.equal(c[:base + n], want[:base + n]) if kv_dtype == 0 else torch.equal(c[:, :base + n], want[:, :base + n])
+        at = torch.tensor(kept, device="cuda")
+        assert torch.equal(q[0, at], chain_q[0])
+        # the chain's attention by the same kernel, whose runs are others (both within their bounds of the definition)
+        chain_out = torch.zeros(1, n, heads * dim, device="cuda")
+        api.attn_tree(_ints([[base, base + n]]), _ints([R.chain(n)]), chain_q, *chain, chain_out, heads, kv, dim, stride, dim ** -0.5,
+                      n, 1, 0, torch.empty_like(ws), kv_dtype=kv_dtype)
+        assert float((chain_out[0] - out[0, at]).abs().max()) <= 4e-5
