@@ -170,7 +170,8 @@ __global__ void __launch_bounds__(256) attn_tree_scalar(TreeParams p) {
 #pragma unroll
         for (int b = 0; b < kB; b++) dst[32 * b + lane] = acc[a][b] * inv;
         if (!whole && lane == 0) {
-            p.part_ml[2 * part] = m[a];
+            // (a maximum leaves out what is not a number; -infinity alone would be a run of which the row sees nothing)
+            p.part_ml[2 * part] = l[a] == l[a] ? m[a] : 0.0f;
             p.part_ml[2 * part + 1] = l[a];
         }
     }
@@ -226,9 +227,7 @@ __global__ void __launch_bounds__(256) attn_tree_fold(TreeParams p) {
             big = most;
 #pragma unroll
             for (int k = 0; k < kAtOnce; k++) {
-                // No run, or one of which the row sees nothing. (By the sum: a maximum leaves out what is not a number, so a
-                // run of nothing but that has -infinity too, and its sum goes on.)
-                if (x[k].y == 0.0f) continue;
+                if (x[k].x == -INFINITY) continue;   // (no run, or one of which the row sees nothing)
                 const float w = exp2f(x[k].x - big);
                 sum.x = fmaf(a[k].x, w, sum.x);
                 sum.y = fmaf(a[k].y, w, sum.y);
@@ -247,8 +246,9 @@ __global__ void __launch_bounds__(256) attn_tree_fold(TreeParams p) {
         sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
         den = 0.0f;
         for (int i = 0; i < groups; i++) {
-            if (s_den[i * cols + col] == 0.0f) continue;
-            const float w = exp2f(s_max[i * cols + col] - big);
+            const float m = s_max[i * cols + col];
+            if (m == -INFINITY) continue;
+            const float w = exp2f(m - big);
             const float4 a = s_sum[i * cols + col];
             sum.x = fmaf(a.x, w, sum.x);
             sum.y = fmaf(a.y, w, sum.y);

@@ -895,7 +895,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tree_tc(TreeParams p) {
             }
             if (live && half == 0 && !whole && !*wait.abort) {
                 const size_t at = 2 * ((size_t)blockIdx.x * kRows + r);
-                p.part_ml[at] = m;
+                p.part_ml[at] = l == l ? m : 0.0f;   // (not a number: -infinity would be a run of which the row sees nothing)
                 p.part_ml[at + 1] = l;
             }
         }
