@@ -75,7 +75,7 @@ __global__ void __launch_bounds__(256) attn_tree_scalar(TreeParams p) {
     const TreeItem it = s_item;
     if (it.slot < 0) return;
     const int rows = min(kRows, it.live * p.group - it.tile * kRows);
-    const int lo = it.first_row(), hi = it.end_row();
+    const unsigned lo = it.first_row(), hi = it.end_row();   // (k0 + 31 below may be past the largest int)
     for (int i = tid; i < it.live; i += 256) s_parents[i] = p.parents[(size_t)it.slot * p.nodes + i];
     const size_t slot_row = (size_t)it.slot * p.nodes;
     // a row of the tile as a row of q and out, in heads
@@ -100,13 +100,12 @@ __global__ void __launch_bounds__(256) attn_tree_scalar(TreeParams p) {
 #pragma unroll
         for (int b = 0; b < kB; b++) acc[a][b] = 0.0f;
     }
-    for (unsigned at = 0; at < (unsigned)(hi - lo); at += kKeys) {
-        const int k0 = lo + (int)at, left = hi - k0;   // (k0 + 31 may be past the largest int)
+    for (unsigned k0 = lo; k0 < hi; k0 += kKeys) {
         __syncthreads();
         for (int i = warp; i < 2 * kB; i += kWarps) {   // lane = cache row: the stores fall into different banks
             const int blk = i % kB;
             float *const dst = (i < kB ? ks : vs) + lane * kPitch + 32 * blk;
-            if (lane < left) {
+            if (k0 + lane < hi) {
                 load_block(p, i < kB ? kc : vc, it.kvh, k0 + lane, blk, dst);
             } else {
 #pragma unroll
@@ -128,8 +127,8 @@ __global__ void __launch_bounds__(256) attn_tree_scalar(TreeParams p) {
         unsigned seen[kWarpRows];   // bit j: the row sees cache row k0 + j
 #pragma unroll
         for (int a = 0; a < kWarpRows; a++) {
-            const int r = warp * kWarpRows + a, drafted = k0 - it.base + lane;
-            bool sees = r < rows && lane < left;
+            const int r = warp * kWarpRows + a, drafted = (int)(k0 + lane - it.base);
+            bool sees = r < rows && k0 + lane < hi;
             if (sees && drafted >= 0) sees = s_sees[r][drafted >> 5] >> (drafted & 31) & 1;
             seen[a] = __ballot_sync(0xffffffffu, sees);
             // (a row that sees nothing of these keeps what it has: -inf - -inf must not be formed)

@@ -63,11 +63,10 @@ __device__ __forceinline__ TreeSlot tree_slot(const int *pos, int slot, int stri
 struct TreeItem {
     int slot, kvh, tile, run, runs;
     int base, live, quota;
-    // the run's rows; nothing beyond the slot's last is formed, which may be the largest int
+    // the run's rows; no row past the slot's last is formed, which may be the largest int
     __device__ __forceinline__ int first_row() const { return run * quota * kTreeKeyTile; }
     __device__ __forceinline__ int end_row() const {
-        const int first = first_row(), rows = base + live - first;
-        return first + (int)min((unsigned)quota * kTreeKeyTile, (unsigned)rows);
+        return run + 1 < runs ? first_row() + quota * kTreeKeyTile : base + live;
     }
 };
 

@@ -5,7 +5,8 @@
 // and r becomes the target row of c; a child that is not kept leaves
 //     r <- max(r - q, 0) / Z,  Z its sum (r stays where Z is 0).
 // Where no child is kept the next token is drawn from r: the first x whose running sum exceeds u_0 times the whole.
-// Accepted tokens and the drawn one are distributed as the target's own (the drafter's errors cost speed only).
+// Accepted tokens and the drawn one are distributed as the target's own (the drafter's errors cost speed only): with draft
+// rows if siblings were drawn from their parent's row independently of one another, without them however they were chosen.
 // No counterpart in the reference, which compares greedy tokens on the host (crates/hipml-model/src/gpu/spec.rs).
 //
 // A slot is one cluster of CTAs; each has a part of the vocabulary, each warp a run of that. What the walk asks of single
