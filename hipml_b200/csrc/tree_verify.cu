@@ -47,11 +47,12 @@ __device__ __forceinline__ double warp_sum_f64(double v) {
     return v;
 }
 
-// The sum of up to four non-negative f32 values, with their rounding errors beside it. The errors themselves are exact and at
-// most 2^-24 of the sum for each add, and as much for all the values; what adding them up loses is at most 21 times 2^-48 of
-// the sum (six errors and the running sums of four, five and six, 2^-24 of each). Sums of more values go on in 64 bits: with
-// 64 fours to a lane less than 2^-43 of the whole is lost. (One such sum for all of a lane's values lost 2^-38 of rows of
-// 2^20 tokens.)
+// The sum of a few non-negative f32 values, with their rounding errors beside it; sums of more go on in 64 bits. The errors
+// are exact and at most 2^-24 of the sum's power of two for each add; what is lost is the rounding of their own running sum,
+// half a last place of 2, 4, 4 and four times 8 of that unit: 21 * 2^-48 of the sum for eight values. Differences come with
+// errors of their own, at most as much as two more such units for all of them: 21 * 2^-48 for four of them (six roundings of
+// 2^-24 of a unit each before they meet, then sums of four, five and six). With the sums in 64 bits less than 2^-43 of the
+// whole is lost, whatever the vocabulary. (One such sum for all of a lane's values lost 2^-38 of rows of 2^20 tokens.)
 struct LongSum {
     float hi = 0.0f, lo = 0.0f;
     __device__ __forceinline__ void add(float x, float error) {
@@ -64,7 +65,6 @@ struct LongSum {
         hi = lo = 0.0f;
     }
 };
-constexpr int kFour = 4;
 
 // grid slots * kCtas, clusters of kCtas.
 template <int kCtas>
@@ -162,16 +162,19 @@ __global__ void __launch_bounds__(kThreads, 2) tree_verify(VerifyParams p) {
                     a[k] = __float_as_uint(a[k]) < 0x7f800000u ? a[k] : 0.0f;
                     b[k] = __float_as_uint(b[k]) < 0x7f800000u ? b[k] : 0.0f;
                 }
+                static_assert(kAtOnce == 8, "eight values, or two times four differences, to a sum");
+                if (!draft) {
 #pragma unroll
-                for (int k = 0; k < kAtOnce; k++) {
-                    if (!draft) {
-                        s.add(a[k], 0.0f);
-                    } else {
+                    for (int k = 0; k < kAtOnce; k++) s.add(a[k], 0.0f);
+                } else {
+#pragma unroll
+                    for (int k = 0; k < kAtOnce; k++) {
                         const float d = a[k] - b[k], e = d - a[k];
                         if (d > 0.0f) s.add(d, (a[k] - (d - e)) - (b[k] + e));
+                        if (k == kAtOnce / 2 - 1) s.move_to(sum);
                     }
-                    if (k % kFour == kFour - 1) s.move_to(sum);
                 }
+                s.move_to(sum);
             }
         } else {
             constexpr int kFew = 4;
