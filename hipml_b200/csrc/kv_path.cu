@@ -31,8 +31,8 @@ __global__ void __launch_bounds__(kThreads) kv_path_keep(const __grid_constant__
         if (tid > 0) before = __ldcg(at - 1);
     }
     const TreeSlot t = tree_slot(p.pos, slot, p.stride, p.nodes);
-    const int count = __ldcg(p.count + slot);
-    if (t.live == 0) return;   // an idle slot: verification has left its path and count as they were
+    const int kept = __ldcg(p.count + slot);
+    const int count = t.live == 0 ? 0 : kept;   // (of an idle slot verification has left path and count as they were)
     bool bad = count < 0 || count > t.live;
     if (tid < count) {
         bad = bad || node <= before || node < 0 || node >= t.live;
