@@ -407,9 +407,9 @@ int sixteen_together() {
 // Clusters of sixteen, which is more than every device must have and is asked for once, as long as all of them fit; more slots
 // take eights (10 slots of 8 nodes of 151,936 with draft rows: 37 us, with eights 60).
 // What bounds it is latency, not memory: a trip for the tree, one for what the walk asks, one pass, the exchange of its sums
-// and the segment of the drawn token follow one another. 8 nodes of 151,936 take 9.9 us, 8 slots of 16 nodes of 50,257 with
-// draft rows 17.5 (several rejections in a row, a pass each), 32 slots of 8 nodes of 151,936 without draft rows 18 (their rows
-// pass in 3).
+// and the segment of the drawn token follow one another. 8 nodes of 151,936 take 9.7 us, 8 slots of 16 nodes of 50,257 with
+// draft rows 14.5 to 20 (rejections in a row, a pass each), 32 slots of 8 nodes of 151,936 without draft rows 18 to 20 (their
+// rows pass in 3).
 int launch_tree_verify(cudaStream_t stream, const VerifyParams &p) {
     static std::atomic<int> sixteen[64];   // one more than clusters; 0: not asked yet
     int dev = 0;

@@ -471,10 +471,10 @@ int hipml_attn_chunk_staged_gated(hipml_stream_t stream, const float *q, float *
  * or hipml_kv_append_chunk_f32 (the first row is a host number there, which a capture keeps).
  *
  * parents is device i32 [slots][nodes]: the parent of node i, an earlier node (< i), or -1. Nothing of
- * a node past a slot's live ones is used or written, whatever the buffers hold there; lengths past the cache count as the cache (hipml_tree_verify knows none:
- * hipml_tree_verify_within). kv_dtype, caches and stride are those of hipml_attn_chunk (0 f32
- * [stride][n_kv*head_dim], 1 q8_0, 2 q4_0 head-major), slot s begins at byte s*kv_slot_bytes (any
- * value where slots is 1). 1..65535 slots. A parent that is no earlier node ends that node's
+ * a node past a slot's live ones is used or written, whatever the buffers hold there; lengths past the
+ * cache count as the cache (hipml_tree_verify knows none: hipml_tree_verify_within). kv_dtype, caches
+ * and stride are those of hipml_attn_chunk (0 f32 [stride][n_kv*head_dim], 1 q8_0, 2 q4_0 head-major),
+ * slot s begins at byte s*kv_slot_bytes (any value where slots is 1). 1..65535 slots. A parent that is no earlier node ends that node's
  * ancestors there and is reported by hipml_check_device_status as 41. The entries here can be captured
  * and replayed: lengths, trees and paths are read on the device. Calls that may overlap on the device
  * must not share a workspace; nothing else is shared between calls.
@@ -482,8 +482,12 @@ int hipml_attn_chunk_staged_gated(hipml_stream_t stream, const float *q, float *
  * Attention of the drafted nodes in one call: node i sees cache rows [0, base), its own row and
  * those of its ancestors. q and out are f32 [slots][nodes][n_heads*head_dim], 16-byte aligned. A row
  * that a node does not see may hold anything, NaN and infinities too, without effect on it.
- * Where it sees a row that is not finite, the heads of that KV head are not finite; rows of f32 caches
- * below 2^-70 lose bits.
+ * Where it sees a row that is not finite, the heads of that KV head are not finite.
+ * head_dim 256 with caches (and kv_slot_bytes, of several slots) on 16 bytes runs on the tensor cores: q,
+ * the values of f32 caches and the weights are taken to 22 bits there (two parts of 11; what a product
+ * of two low parts would add, 2^-22 of it, is left out), q8_0 and q4_0 values are exact, sums are f32;
+ * rows of f32 caches below 2^-70 lose more. Other head sizes and alignments are f32 throughout, on the
+ * CUDA cores, which takes some fifteen times as long over long caches: align them.
  * workspace: hipml_attn_tree_workspace_bytes(...) bytes on 16 (0: the arguments are refused; it
  * depends on the current device's SMs). */
 size_t hipml_attn_tree_workspace_bytes(int n_heads, int n_kv, int head_dim, int nodes, int slots);
@@ -502,16 +506,20 @@ int hipml_attn_tree(hipml_stream_t stream, int kv_dtype, const int *pos, const i
  * x, 0 elsewhere); otherwise r becomes max(r - q, 0) over its sum (and stays where that is 0). Where
  * no child is kept, `next` is the lowest token whose running sum of r exceeds uniform[0] times
  * the whole (the last token with r > 0 where rounding leaves none; -1 where r has no mass). path i32
- * [slots][nodes] receives the kept nodes in order, then -1; count i32 [slots] how many. Outputs of a
+ * [slots][nodes] receives the kept nodes in order, then -1; count i32 [slots] how many. The tokens that a
+ * step emits are distributed as the target's own if the children of a node were drawn from its draft
+ * row independently of one another (a token may come twice), and without draft rows however they were
+ * chosen, as long as it was without regard to uniform: the k best of a drafter, or what it drew
+ * without replacement, are passed with draft NULL. Outputs of a
  * slot without live nodes stay as they are. Sums are exact to 2^-43. What is no probability (NaN,
  * negative, infinite) counts as 0; a child whose parent is no earlier node or whose token is not in
  * the vocabulary is never kept (device status 41). vocab 1..1048576. */
 int hipml_tree_verify(hipml_stream_t stream, const int *pos, const int *parents, const int *tokens,
                       const float *target, const float *draft, const float *uniform, int *path,
                       int *count, int *next, int nodes, int slots, int vocab, long long row_stride);
-/* The same over the nodes that a cache of `stride` rows holds: those of a tree that crosses its end which attention and
- * the kept path leave out are not kept, and nothing of their rows is read. hipml_tree_verify knows no cache: there
- * base + live nodes has to lie within it. */
+/* The same over the nodes that a cache of `stride` rows holds: those of a tree that crosses its end
+ * which attention and the kept path leave out are not kept, and nothing of their rows is read.
+ * hipml_tree_verify knows no cache: there base + live nodes has to lie within it. */
 int hipml_tree_verify_within(hipml_stream_t stream, const int *pos, const int *parents, const int *tokens,
                              const float *target, const float *draft, const float *uniform, int *path,
                              int *count, int *next, int nodes, int slots, int vocab, long long row_stride,
@@ -520,9 +528,9 @@ int hipml_tree_verify_within(hipml_stream_t stream, const int *pos, const int *p
 /* The kept path's cache rows move together behind the prefix: in every cache of `layers` layers row
  * base + path[i] becomes row base + i, i < count (path and count as hipml_tree_verify leaves them; the
  * other rows stay). k_caches and v_caches are HOST arrays of `layers` device pointers, all different.
- * A path must ascend and stay among the live nodes: otherwise the slot is left as it was (device status 42). A slot
- * without live nodes is left as it was whatever its path and count hold, which is what verification leaves there.
- * One launch for up to 64 layers; cache addresses are taken at the call. */
+ * A path must ascend and stay among the live nodes: otherwise the slot is left as it was (device status
+ * 42). A slot without live nodes is left as it was whatever its path and count hold: verification
+ * leaves those of the step before there. One launch for up to 64 layers; cache addresses are taken at the call. */
 int hipml_kv_path_keep(hipml_stream_t stream, int kv_dtype, const int *pos, const int *path,
                        const int *count, void *const *k_caches, void *const *v_caches, int layers,
                        int n_kv, int head_dim, int stride, int nodes, int slots, size_t kv_slot_bytes);
