@@ -7,6 +7,7 @@
 #include <cstring>
 
 #include "common.cuh"
+#include "tree.cuh"
 
 namespace hipml {
 
@@ -250,7 +251,10 @@ int hipml_check_device_status(hipml_stream_t stream, int *status) {
     if (value != 0) {
         const int zero = 0;
         cudaMemcpy(word, &zero, sizeof(int), cudaMemcpyHostToDevice);
-        return fail(HIPML_ERR_DEVICE_STATUS, "a kernel's bounded wait ran out (code %d)", value);
+        const char *const what = value == kTreeBadTree   ? "a tree has a parent that is no earlier node, or a token past the vocabulary"
+                                 : value == kTreeBadPath ? "a kept path does not ascend within its tree"
+                                                         : "a kernel's bounded wait ran out";
+        return fail(HIPML_ERR_DEVICE_STATUS, "%s (code %d)", what, value);
     }
     return HIPML_SUCCESS;
 }

@@ -474,15 +474,16 @@ int hipml_attn_chunk_staged_gated(hipml_stream_t stream, const float *q, float *
  * a node past a slot's live ones is used or written, whatever the buffers hold there; lengths past the
  * cache count as the cache (hipml_tree_verify knows none: hipml_tree_verify_within). kv_dtype, caches
  * and stride are those of hipml_attn_chunk (0 f32 [stride][n_kv*head_dim], 1 q8_0, 2 q4_0 head-major),
- * slot s begins at byte s*kv_slot_bytes (any value where slots is 1). 1..65535 slots. A parent that is no earlier node ends that node's
- * ancestors there and is reported by hipml_check_device_status as 41. The entries here can be captured
- * and replayed: lengths, trees and paths are read on the device. Calls that may overlap on the device
- * must not share a workspace; nothing else is shared between calls.
+ * slot s begins at byte s*kv_slot_bytes (any value where slots is 1). 1..65535 slots. A parent that is
+ * no earlier node ends that node's ancestors there and is reported by hipml_check_device_status as 41.
+ * The entries here can be captured and replayed: lengths, trees and paths are read on the device. Calls
+ * that may overlap on the device must not share a workspace; nothing else is shared between calls.
  *
  * Attention of the drafted nodes in one call: node i sees cache rows [0, base), its own row and
  * those of its ancestors. q and out are f32 [slots][nodes][n_heads*head_dim], 16-byte aligned. A row
  * that a node does not see may hold anything, NaN and infinities too, without effect on it.
- * Where it sees a row that is not finite, the heads of that KV head are not finite.
+ * Where it sees a row that is not finite, the heads of that KV head are not finite: all of their values,
+ * or, of a V row on the CUDA cores (below), those dims at least that are not finite in it.
  * head_dim 256 with caches (and kv_slot_bytes, of several slots) on 16 bytes runs on the tensor cores: q,
  * the values of f32 caches and the weights are taken to 22 bits there (two parts of 11; what a product
  * of two low parts would add, 2^-22 of it, is left out), q8_0 and q4_0 values are exact, sums are f32;
@@ -556,7 +557,7 @@ int hipml_set_decode_fold_mode(int mode);
 int hipml_decode_plan_quota(const int *lens, int slots, int splits, int n_kv, int cta_slots);
 
 /* Reads and clears the device status word that kernels with bounded waits set when a wait
- * ran out (0 = none). Synchronises `stream`. Returns HIPML_ERR_DEVICE_STATUS if it was set. */
+ * ran out, and the entries of tree speculation for a tree or path that is none (0 = none). Synchronises `stream`. Returns HIPML_ERR_DEVICE_STATUS if it was set. */
 int hipml_check_device_status(hipml_stream_t stream, int *status);
 
 /* Library build identification: "hipml_cuda <version> sm_100a". */

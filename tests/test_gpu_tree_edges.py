@@ -4,7 +4,7 @@ import numpy as np
 import pytest
 import torch
 
-from hipml_b200 import api
+from hipml_b200 import _lib, api
 from tests import tree_reference as R
 from tests.test_gpu_tree import Step, _dev, _ints, _spoil, status  # noqa: F401 (status: every test leaves the device's clear)
 
@@ -304,3 +304,14 @@ def test_a_captured_step_of_a_branching_tree_with_rotated_rows(kv_dtype):
         api.attn_tree(_ints([[base, base + n]]), _ints([R.chain(n)]), chain_q, *chain, chain_out, heads, kv, dim, stride, dim ** -0.5,
                       n, 1, 0, torch.empty_like(ws), kv_dtype=kv_dtype)
         assert float((chain_out[0] - out[0, at]).abs().max()) <= 4e-5
+
+
+def test_the_status_names_what_was_wrong():
+    step = Step(10, 1, [(20, 3, [-1, 0, 5])], 3, heads=2, kv=1, dim=64)
+    step.call()
+    with pytest.raises(_lib.HipmlError, match="no earlier node.*41"):
+        api.check_device_status()
+    cache = torch.zeros(2, 30, 68, dtype=torch.uint8, device="cuda")
+    api.kv_path_keep(_ints([[20, 23]]), _ints([[1, 0, -1]]), _ints([2]), [cache], [cache.clone()], 2, 64, 30, 3, 1, 0)
+    with pytest.raises(_lib.HipmlError, match="does not ascend.*42"):
+        api.check_device_status()
